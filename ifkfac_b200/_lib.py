@@ -22,6 +22,7 @@ F32, BF16 = 0, 1
 PREC_AUTO, PREC_FP32, PREC_BF16 = 0, 1, 2
 FOLD_TRAPEZOIDAL_CHUNK = 1
 FOLD_DEBUG_WITHHOLD = 256  # tests of the failure path only
+Q8_GROUP = 32
 
 _i64, _sz, _vp, _int, _dbl = ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_int, ctypes.c_double
 
@@ -66,6 +67,17 @@ SIGNATURES = {
     "ifk_update_workspace": (_sz, [_i64]),
     "ifk_update": (_int, [_vp, _vp, _vp, _i64, _dbl, _dbl, _dbl, _dbl, _int, _vp, _sz, _vp]),
     "ifk_update_bias": (_int, [_vp, _vp, _i64, _dbl, _dbl, _vp]),
+    "ifk_q8_pitch": (_i64, [_i64]),
+    "ifk_q8_quantize": (_int, [_vp, _i64, _int, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "ifk_q8_dequantize": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp]),
+    "ifk_q8_wgrad_workspace": (_sz, [_i64, _i64, _i64, _int]),
+    "ifk_q8_wgrad": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _int, _vp,
+                            _vp, _sz, _vp]),
+    "ifk_layernorm": (_int, [_vp, _i64, _int, _vp, _vp, _int, _i64, _i64, _dbl, _vp, _i64, _int, _vp, _vp, _vp,
+                             _i64, _vp, _i64, _vp]),
+    "ifk_layernorm_backward_workspace": (_sz, [_i64, _i64]),
+    "ifk_layernorm_backward": (_int, [_vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _int,
+                                      _i64, _i64, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

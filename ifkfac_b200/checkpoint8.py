@@ -1,0 +1,455 @@
+"""Activations held in 8 bits, the products that read them, and layer norm.
+
+The rows that a training step keeps for later (a Linear layer's input for its
+weight gradient and for the Kronecker factor, a layer norm's input for its
+backward pass) can be held as :class:`Q8Rows`: one byte an element and one a
+group of 32 columns, in the format of ``include/ifk.h`` (a power-of-two scale a
+group and integer codes, so every value is exact in bf16 and fp32).
+
+* :func:`quantize_rows` / :func:`dequantize_rows`: rows to 8 bits and back,
+  optionally a gather of rows (the hooks' random row subsample);
+* :func:`weight_grad`: dW = delta^T X and db from the 8-bit rows of X;
+* :func:`layer_norm_forward` / :func:`layer_norm_backward`: layer norm with its
+  weight and bias gradients, from the saved input or its 8-bit rows;
+* :class:`Linear8`, :class:`LayerNorm8`: ``nn.Linear`` / ``nn.LayerNorm`` that
+  save their input in 8 bits for the backward pass, and :func:`convert`, which
+  puts them in a model's place of its own.
+
+``RawActivationHooks(capture_8bit=True)`` (and ``IFKFAC``) keeps its pending rows
+this way; next to a :class:`Linear8` it shares that layer's rows.
+
+Everything runs in libifk.so on CUDA tensors (fp32 or bf16); there is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _lib
+from ._lib import check
+
+__all__ = ["Q8Rows", "quantize_rows", "dequantize_rows", "weight_grad", "LayerNormSaved", "layer_norm_forward",
+           "layer_norm_backward", "Linear8", "LayerNorm8", "convert"]
+
+_DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_G = _lib.Q8_GROUP
+
+
+def _code(dtype: torch.dtype) -> int:
+    try:
+        return _DT[dtype]
+    except KeyError:
+        raise TypeError(f"ifkfac_b200 supports float32 and bfloat16 tensors, got {dtype}") from None
+
+
+def _need_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The one CUDA device of the tensors (None entries are skipped)."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("ifkfac_b200 operates on CUDA tensors only (no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one call works on one device")
+    return dev
+
+
+class _On:
+    """The device of a call made current, where it is not already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, dev: torch.device):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
+    """Row-major with unit column stride (leading dimension = stride(0))."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D rows, got shape {tuple(t.shape)}")
+    if t.shape[1] == 0:
+        raise ValueError(f"{what} has no columns")
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Leading dimension; a single row's stride is not used and may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class Q8Rows:
+    """Rows in 8 bits: ``codes`` (rows x pitch int8, pitch = ``cols`` rounded up to a
+    multiple of 32), ``scales`` (rows x pitch / 32 uint8).  Slices along the rows are
+    views of the same storage."""
+
+    __slots__ = ("codes", "scales", "cols")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
+        cols = int(cols)
+        pitch = -(-cols // _G) * _G
+        if cols < 1 or codes.dim() != 2 or scales.dim() != 2 or codes.shape != (scales.shape[0], pitch) \
+                or scales.shape[1] != pitch // _G:
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not rows of {cols} "
+                             f"columns (rows x {pitch} and rows x {pitch // _G})")
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise TypeError(f"8-bit rows are int8 codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+        if codes.shape[0] > 1 and (codes.stride(0) < pitch or scales.stride(0) < pitch // _G) \
+                or codes.stride(1) != 1 or (scales.stride(1) != 1 and scales.shape[1] > 1):
+            raise ValueError("codes and scales must be row-major")
+        self.codes, self.scales, self.cols = codes, scales, cols
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device) -> "Q8Rows":
+        pitch = -(-int(cols) // _G) * _G
+        return cls(torch.empty(rows, pitch, dtype=torch.int8, device=device),
+                   torch.empty(rows, pitch // _G, dtype=torch.uint8, device=device), cols)
+
+    @property
+    def rows(self) -> int:
+        return int(self.codes.shape[0])
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.rows * (self.codes.shape[1] + self.scales.shape[1])
+
+    def __getitem__(self, rows: slice) -> "Q8Rows":
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("8-bit rows are sliced along the rows, with step 1")
+        return Q8Rows(self.codes[rows], self.scales[rows], self.cols)
+
+    def __repr__(self) -> str:
+        return f"Q8Rows({self.rows} x {self.cols}, {self.device})"
+
+
+def _index(index: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]:
+    if index is None:
+        return None
+    if index.dim() != 1 or index.dtype not in (torch.int64, torch.int32):
+        raise ValueError("a row index is a 1-D integer tensor")
+    return index.to(device=dev, dtype=torch.int64).contiguous()
+
+
+def _q8(q: Q8Rows):
+    """(codes, ld, scales, ld) of a call's arguments."""
+    return q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(), _ld(q.scales)
+
+
+def quantize_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None,
+                  status: Optional[torch.Tensor] = None) -> Q8Rows:
+    """The 8-bit rows of ``x`` (rows x cols, fp32 or bf16), or of its rows ``index``.
+
+    Per group of 32 columns with largest magnitude a, the error is at most a / 64; a
+    group that holds a NaN or an infinity reads back as NaN.  An index outside x
+    gives a zero row and IFK_ERR_ARG in ``status`` (a device int32, optional)."""
+    dev = _need_cuda(x, status)
+    x = _rows2d(x, "x")
+    dt = _code(x.dtype)
+    index = _index(index, dev)
+    rows = x.shape[0] if index is None else index.numel()
+    with _On(dev) as stream:
+        q = Q8Rows.empty(rows, x.shape[1], dev)
+        check(_lib.lib().ifk_q8_quantize(x.data_ptr(), _ld(x), dt, _ptr(index), x.shape[0], rows, x.shape[1], *_q8(q),
+                                         _ptr(status), stream), "ifk_q8_quantize")
+    return q
+
+
+def dequantize_rows(q: Q8Rows, dtype: torch.dtype = torch.bfloat16, index: Optional[torch.Tensor] = None,
+                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values of 8-bit rows (or of the rows ``index`` of them), exact in either dtype."""
+    dev = _need_cuda(q.codes, q.scales, status)
+    dt = _code(dtype)
+    index = _index(index, dev)
+    rows = q.rows if index is None else index.numel()
+    with _On(dev) as stream:
+        out = torch.empty(rows, q.cols, dtype=dtype, device=dev)
+        check(_lib.lib().ifk_q8_dequantize(*_q8(q), _ptr(index), q.rows, rows, q.cols, out.data_ptr(), q.cols, dt,
+                                           _ptr(status), stream), "ifk_q8_dequantize")
+    return out
+
+
+def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optional[torch.Tensor] = None,
+                out_bias: Optional[torch.Tensor] = None, accumulate: bool = False,
+                status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(dW, db) of a linear layer y = x W^T + b: dW = delta^T X (n_out x n_in fp32)
+    from the 8-bit rows of X, and with ``bias`` (or ``out_bias``) db = the column sums
+    of delta, else None.  ``out`` / ``out_bias`` receive them; with ``accumulate`` they
+    are added to (gradient accumulation), and both that are wanted must be given."""
+    dev = _need_cuda(delta, q.codes, q.scales, out, out_bias, status)
+    delta = _rows2d(delta, "delta")
+    dt = _code(delta.dtype)
+    rows, n_out = delta.shape
+    if rows != q.rows:
+        raise ValueError(f"delta has {rows} rows, the layer's input {q.rows}")
+    if accumulate and (out is None or (bias and out_bias is None)):
+        raise ValueError("accumulate needs the tensors to add to")
+    with _On(dev) as stream:
+        if out is None:
+            out = torch.empty(n_out, q.cols, dtype=torch.float32, device=dev)
+        elif out.dtype != torch.float32 or out.shape != (n_out, q.cols) or out.stride(1) != 1 \
+                or (n_out > 1 and out.stride(0) < q.cols):
+            raise ValueError(f"out must be a row-major {n_out} x {q.cols} float32 tensor")
+        if out_bias is None and bias:
+            out_bias = torch.empty(n_out, dtype=torch.float32, device=dev)
+        elif out_bias is not None and (out_bias.dtype != torch.float32 or out_bias.shape != (n_out,)
+                                       or not out_bias.is_contiguous()):
+            raise ValueError(f"out_bias must be a contiguous float32 tensor of {n_out}")
+        L = _lib.lib()
+        ws = torch.empty(L.ifk_q8_wgrad_workspace(rows, n_out, q.cols, dt), dtype=torch.uint8, device=dev)
+        check(L.ifk_q8_wgrad(delta.data_ptr(), _ld(delta), dt, *_q8(q), rows, n_out, q.cols, out.data_ptr(), _ld(out),
+                             _ptr(out_bias), 1 if accumulate else 0, _ptr(status), ws.data_ptr(), ws.numel(), stream),
+              "ifk_q8_wgrad")
+    return out, out_bias
+
+
+class LayerNormSaved:
+    """What layer norm's backward pass needs of its forward pass: the statistics and
+    the input rows, as they were (``x``) or in 8 bits (``q8``)."""
+
+    __slots__ = ("x", "q8", "mean", "rstd", "x_dtype", "cols")
+
+    def __init__(self, x, q8, mean, rstd, x_dtype, cols):
+        self.x, self.q8, self.mean, self.rstd, self.x_dtype, self.cols = x, q8, mean, rstd, x_dtype, cols
+
+
+def _affine(n: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must hold {n} contiguous values, got shape {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias share a dtype, got {weight.dtype} and {bias.dtype}")
+    t = weight if weight is not None else bias
+    return _lib.F32 if t is None else _code(t.dtype)
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5, out_dtype: Optional[torch.dtype] = None, save: bool = False,
+                       checkpoint: bool = False) -> Tuple[torch.Tensor, Optional[LayerNormSaved]]:
+    """y = (x - mean) * rstd * weight + bias over the columns of ``x`` (rows x cols),
+    in ``out_dtype`` (x's by default).  With ``save`` the second value holds what
+    :func:`layer_norm_backward` needs; with ``checkpoint`` the input is held there
+    in 8 bits, written in the same pass, instead of as itself."""
+    dev = _need_cuda(x, weight, bias)
+    x = _rows2d(x, "x")
+    dt = _code(x.dtype)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    ydt = _code(out_dtype)
+    rows, n = x.shape
+    wdt = _affine(n, weight, bias)
+    saved = mean = rstd = None
+    q = (None, 0, None, 0)
+    with _On(dev) as stream:
+        y = torch.empty(rows, n, dtype=out_dtype, device=dev)
+        if save:
+            mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=dev)
+            rows8 = Q8Rows.empty(rows, n, dev) if checkpoint else None
+            saved = LayerNormSaved(None if checkpoint else x, rows8, mean, rstd, x.dtype, n)
+            if checkpoint:
+                q = _q8(rows8)
+        check(_lib.lib().ifk_layernorm(x.data_ptr(), _ld(x), dt, _ptr(weight), _ptr(bias), wdt, rows, n, float(eps),
+                                       y.data_ptr(), n, ydt, _ptr(mean), _ptr(rstd), *q, stream), "ifk_layernorm")
+    return y, saved
+
+
+def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optional[torch.Tensor] = None,
+                        weight_grads: bool = True
+                        ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dw, db) of :func:`layer_norm_forward`: dx in the input's dtype, dw and db
+    fp32 (None without ``weight_grads``)."""
+    dev = _need_cuda(dy, saved.mean, weight)
+    dy = _rows2d(dy, "dy")
+    dt, xdt = _code(dy.dtype), _code(saved.x_dtype)
+    rows, n = dy.shape
+    if (rows, n) != (saved.mean.numel(), saved.cols):
+        raise ValueError(f"dy is {rows} x {n}, the input was {saved.mean.numel()} x {saved.cols}")
+    wdt = _affine(n, weight, None)
+    x, q = saved.x, (None, 0, None, 0)
+    if x is None:
+        q = _q8(saved.q8)
+    with _On(dev) as stream:
+        L = _lib.lib()
+        dx = torch.empty(rows, n, dtype=saved.x_dtype, device=dev)
+        dw = db = ws = None
+        if weight_grads:
+            dw, db = torch.empty(2, n, dtype=torch.float32, device=dev)
+            ws = torch.empty(L.ifk_layernorm_backward_workspace(rows, n), dtype=torch.uint8, device=dev)
+        check(L.ifk_layernorm_backward(
+            dy.data_ptr(), _ld(dy), dt, _ptr(x), 0 if x is None else _ld(x), xdt, *q, saved.mean.data_ptr(),
+            saved.rstd.data_ptr(), _ptr(weight), wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(ws),
+            0 if ws is None else ws.numel(), stream), "ifk_layernorm_backward")
+    return dx, dw, db
+
+
+# ---- autograd and modules ----
+
+def _autocast_dtype() -> Optional[torch.dtype]:
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+
+
+class _LinearQ8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, dtype, q):
+        with torch.autocast("cuda", enabled=False):
+            w = weight.to(dtype)
+            y = F.linear(x.to(dtype), w, None if bias is None else bias.to(dtype))
+        saved = [] if q is None else [q.codes, q.scales]
+        ctx.save_for_backward(w, *saved)
+        ctx.cols, ctx.x_shape, ctx.x_dtype = x.shape[-1], x.shape, x.dtype
+        ctx.w_dtype, ctx.b_dtype = weight.dtype, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w, *saved = ctx.saved_tensors
+        dx = dw = db = None
+        with torch.autocast("cuda", enabled=False):
+            d2 = dy.reshape(-1, dy.shape[-1])
+            if ctx.needs_input_grad[0]:
+                dx = (d2 @ w).reshape(ctx.x_shape).to(ctx.x_dtype)
+            if ctx.needs_input_grad[1]:
+                dw, db = weight_grad(d2, Q8Rows(*saved, ctx.cols), bias=ctx.needs_input_grad[2])
+                dw = dw.to(ctx.w_dtype)
+                db = None if db is None else db.to(ctx.b_dtype)
+            elif ctx.needs_input_grad[2]:
+                db = d2.sum(0, dtype=torch.float32).to(ctx.b_dtype)
+        return dx, dw, db, None, None
+
+
+class Linear8(nn.Linear):
+    """``nn.Linear`` that keeps its input in 8 bits for the weight gradient.
+
+    Forward and input gradient are ``nn.Linear``'s (in the autocast dtype under
+    autocast); the weight and bias gradients come from :func:`weight_grad`, summed in
+    fp32.  While hooks that capture in 8 bits are attached, ``take_rows`` hands them
+    the rows of the last forward pass, so they are quantised once."""
+
+    _share_rows = False   # set by the hooks that want the rows
+    _last_rows: Optional[Q8Rows] = None
+
+    @classmethod
+    def from_linear(cls, m: nn.Linear) -> "Linear8":
+        """A Linear8 on the parameters of ``m``."""
+        new = cls(m.in_features, m.out_features, bias=m.bias is not None, device="meta")
+        new.weight, new.bias, new.training = m.weight, m.bias, m.training
+        return new
+
+    def take_rows(self) -> Optional[Q8Rows]:
+        rows, self._last_rows = self._last_rows, None
+        return rows
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _need_cuda(x, self.weight, self.bias)
+        dtype = _autocast_dtype() or self.weight.dtype
+        _code(dtype)
+        if dtype != x.dtype and not torch.is_autocast_enabled("cuda"):
+            raise TypeError(f"input {x.dtype} and weight {self.weight.dtype} differ")
+        q = None
+        if torch.is_grad_enabled() and self.weight.requires_grad:
+            q = quantize_rows(x.detach().reshape(-1, x.shape[-1]))
+            if self._share_rows:
+                self._last_rows = q
+        return _LinearQ8.apply(x, self.weight, self.bias, dtype, q)
+
+
+class _LayerNormQ8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, dtype, save):
+        y, s = layer_norm_forward(x.reshape(-1, x.shape[-1]), weight, bias, eps, dtype, save=save, checkpoint=True)
+        if s is not None:
+            ctx.save_for_backward(s.mean, s.rstd, s.q8.codes, s.q8.scales, *(() if weight is None else (weight,)))
+        ctx.x_dtype, ctx.x_shape = x.dtype, x.shape
+        ctx.b_dtype = None if bias is None else bias.dtype
+        return y.reshape(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        mean, rstd, codes, scales, *w = ctx.saved_tensors
+        n = ctx.x_shape[-1]
+        saved = LayerNormSaved(None, Q8Rows(codes, scales, n), mean, rstd, ctx.x_dtype, n)
+        weight = w[0] if w else None
+        dx, dw, db = layer_norm_backward(dy.reshape(-1, n), saved, weight,
+                                         weight_grads=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return (dx.reshape(ctx.x_shape) if ctx.needs_input_grad[0] else None,
+                dw.to(weight.dtype) if ctx.needs_input_grad[1] else None,
+                db.to(ctx.b_dtype) if ctx.needs_input_grad[2] else None, None, None, None)
+
+
+class LayerNorm8(nn.LayerNorm):
+    """``nn.LayerNorm`` over the last dimension that keeps its input in 8 bits for the
+    backward pass.  The output has the input's dtype, or the autocast dtype under
+    autocast (the Linear layers that read it would cast it)."""
+
+    def __init__(self, normalized_shape, *args, **kwargs):
+        super().__init__(normalized_shape, *args, **kwargs)
+        if len(self.normalized_shape) != 1:
+            raise ValueError(f"LayerNorm8 normalises the last dimension, got {tuple(self.normalized_shape)}")
+
+    @classmethod
+    def from_layer_norm(cls, m: nn.LayerNorm) -> "LayerNorm8":
+        """A LayerNorm8 on the parameters of ``m``."""
+        new = cls(m.normalized_shape, eps=m.eps, elementwise_affine=m.elementwise_affine, bias=m.bias is not None,
+                  device="meta")
+        new.weight, new.bias, new.training = m.weight, m.bias, m.training
+        return new
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"input of width {x.shape[-1]} for a layer norm of {self.normalized_shape[0]}")
+        dtype = _autocast_dtype() or x.dtype
+        params = [p for p in (x, self.weight, self.bias) if p is not None]
+        save = torch.is_grad_enabled() and any(p.requires_grad for p in params)
+        return _LayerNormQ8.apply(x, self.weight, self.bias, self.eps, dtype, save)
+
+
+def convert(model: nn.Module, linear: bool = True, layer_norm: bool = True) -> nn.Module:
+    """``model`` with each nn.Linear (``linear``) and each nn.LayerNorm over one dimension
+    (``layer_norm``) replaced, in place, by :class:`Linear8` / :class:`LayerNorm8` on
+    the same parameters.  Subclasses, and layers that already carry hooks, are left as
+    they are: convert before an optimizer attaches its hooks.  A model that is itself
+    such a layer is returned replaced."""
+
+    def swap(m: nn.Module) -> nn.Module:
+        if m._forward_hooks or m._backward_hooks or m._forward_pre_hooks or m._backward_pre_hooks:
+            return m
+        if linear and type(m) is nn.Linear:
+            return Linear8.from_linear(m)
+        if layer_norm and type(m) is nn.LayerNorm and len(m.normalized_shape) == 1:
+            return LayerNorm8.from_layer_norm(m)
+        return m
+
+    done = {}
+    for parent in list(model.modules()):
+        for name, child in list(parent._modules.items()):
+            if child is None:
+                continue
+            if child not in done:  # a layer used in two places stays one layer
+                done[child] = swap(child)
+            if done[child] is not child:
+                parent._modules[name] = done[child]
+    return swap(model)

@@ -176,4 +176,28 @@ int update_run(float* W, float* buf, const float* nat, int64_t count, double lr,
 int update_bias_run(float* b, const float* nat, int64_t count, double lr, double wd,
                     cudaStream_t s);
 
+// 8-bit activation rows (q8.cu, q8_wgrad.cu) and layer norm (layernorm.cu).  Row
+// index and status as in copy_chunk; vectors of partial sums are parts x n.
+int q8_quantize_run(const void* x, int64_t ldx, int dtype, const int64_t* ridx, int64_t src_rows, int64_t rows,
+                    int64_t n, int8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, int* status,
+                    cudaStream_t s);
+int q8_dequantize_run(const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const int64_t* ridx,
+                      int64_t src_rows, int64_t rows, int64_t n, void* out, int64_t ldo, int dtype, int* status,
+                      cudaStream_t s);
+size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype);
+int q8_wgrad_run(const void* delta, int64_t ldd, int dtype, const int8_t* codes, int64_t ldc, const uint8_t* scales,
+                 int64_t lds, int64_t rows, int64_t n_out, int64_t n_in, float* dW, int64_t ldw, float* db,
+                 int accumulate, int* status, uint8_t* ws, cudaStream_t s);
+int layernorm_run(const void* x, int64_t ldx, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,
+                  int64_t n, double eps, void* y, int64_t ldy, int y_dtype, float* mean, float* rstd, int8_t* codes,
+                  int64_t ldc, uint8_t* scales, int64_t lds, cudaStream_t s);
+size_t layernorm_backward_bytes(int64_t rows, int64_t n);
+int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype,
+                           const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const float* mean,
+                           const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n, void* dx,
+                           int64_t lddx, float* dw, float* db, float* part, cudaStream_t s);
+// out = sum over the parts of part (parts x n), in a fixed order; likewise part2 into out2 (a null out is skipped)
+int sum_parts_run(const float* part, int64_t parts, int64_t n, float* out, const float* part2, float* out2,
+                  int accumulate, cudaStream_t s);
+
 }  // namespace ifk

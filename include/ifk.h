@@ -472,6 +472,96 @@ IFK_API int ifk_update(float* W, float* buf, const float* nat, int64_t count,
 IFK_API int ifk_update_bias(float* b, const float* nat_b, int64_t count, double lr,
                     double weight_decay, ifk_stream_t stream);
 
+/* ---- 8-bit activation rows ------------------------------------------------ */
+
+/*
+ * Rows of activations (or gradients) held in 8 bits: a row's columns in groups
+ * of IFK_Q8_GROUP = 32 share one power-of-two scale.  With a the largest |x| of
+ * a group, e = floor(log2 a) - 6 (at least -126, at most 121; -126 when a = 0),
+ * the scale byte is e + 127 and column j's code is x_j 2^-e rounded to the
+ * nearest integer (ties to even) and clipped to [-127, 127]; its value is
+ * code * 2^e.  The error is at most 2^e <= a / 64 (half of that where the code
+ * is not clipped), and a value has at most 7 significant bits, so it is exact in
+ * bf16 and fp32.  A group with a NaN or an infinity has scale byte 255 and codes
+ * 0: all its values read as NaN.
+ *
+ * codes is rows x ld_codes int8 with ld_codes >= ifk_q8_pitch(n) (n rounded up
+ * to a multiple of 32; the columns past n are written as 0 and never used), a
+ * multiple of 16, and a 16-byte aligned base; scales is rows x ld_scales uint8
+ * with ld_scales >= ifk_q8_pitch(n) / 32.  The reference keeps such rows in
+ * the dtype they were captured in (ifkfac/activation_hooks.py:560-570, 627-635).
+ */
+#define IFK_Q8_GROUP 32
+IFK_API int64_t ifk_q8_pitch(int64_t n);
+
+/*
+ * Quantise `rows` rows of n columns of x (element type dtype, leading dimension
+ * ld_x).  Row i is row row_index[i] of x when row_index (a device array of
+ * `rows` int64) is given: src_rows is then x's row count, and an index outside
+ * [0, src_rows) gives a zero row and sets IFK_ERR_ARG in *d_status (may be NULL).
+ */
+IFK_API int ifk_q8_quantize(const void* x, int64_t ld_x, int dtype, const int64_t* row_index,
+                            int64_t src_rows, int64_t rows, int64_t n, int8_t* codes, int64_t ld_codes,
+                            uint8_t* scales, int64_t ld_scales, int* d_status, ifk_stream_t stream);
+
+/* The values of `rows` rows (row_index, src_rows as above, into the 8-bit rows),
+ * exact in either out_dtype. */
+IFK_API int ifk_q8_dequantize(const int8_t* codes, int64_t ld_codes, const uint8_t* scales,
+                              int64_t ld_scales, const int64_t* row_index, int64_t src_rows,
+                              int64_t rows, int64_t n, void* out, int64_t ld_out, int out_dtype,
+                              int* d_status, ifk_stream_t stream);
+
+/* Workspace bytes for ifk_q8_wgrad (with or without db). */
+IFK_API size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in, int delta_dtype);
+
+/*
+ * Gradients of a linear layer y = x W^T + b from its 8-bit input rows:
+ *   dW = delta^T X  (n_out x n_in fp32),   db = column sums of delta (n_out fp32; NULL: not formed),
+ * with X the values of the 8-bit rows (rows x n_in) and delta rows x n_out
+ * (bf16 or fp32).  accumulate != 0 adds to dW and db instead of overwriting
+ * them.  The products are exact and summed in fp32 in either delta type (an fp32
+ * delta is taken apart into three bf16 terms); the result does not depend on
+ * the run.  rows == 0 gives zeros (or adds nothing).  *d_status (may be NULL)
+ * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up.
+ */
+IFK_API int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int8_t* codes,
+                         int64_t ld_codes, const uint8_t* scales, int64_t ld_scales, int64_t rows,
+                         int64_t n_out, int64_t n_in, float* dW, int64_t ld_dW, float* db, int accumulate,
+                         int* d_status, void* workspace, size_t workspace_bytes, ifk_stream_t stream);
+
+/* ---- layer norm -------------------------------------------------------------- */
+
+/*
+ * y = (x - mu) r w + b per row, mu = mean(x), r = (mean((x - mu)^2) + eps)^-1/2,
+ * statistics in fp32.  x: rows x n (x_dtype), y: rows x n (y_dtype); w and b hold
+ * n values of w_dtype, or are NULL (1 and 0).  mean and rstd (rows fp32) receive
+ * the statistics (NULL: not stored).  With codes and scales (both or neither),
+ * the 8-bit rows of x are written in the same pass, bit for bit those of
+ * ifk_q8_quantize.
+ */
+IFK_API int ifk_layernorm(const void* x, int64_t ld_x, int x_dtype, const void* w, const void* b,
+                          int w_dtype, int64_t rows, int64_t n, double eps, void* y, int64_t ld_y,
+                          int y_dtype, float* mean, float* rstd, int8_t* codes, int64_t ld_codes,
+                          uint8_t* scales, int64_t ld_scales, ifk_stream_t stream);
+
+/* Workspace bytes for ifk_layernorm_backward. */
+IFK_API size_t ifk_layernorm_backward_workspace(int64_t rows, int64_t n);
+
+/*
+ * Gradients of ifk_layernorm: with z = (x - mean) rstd and g = dy w,
+ *   dx = rstd (g - mean(g) - z mean(g z))   (rows x n, x_dtype),
+ *   dw = sum over rows of dy z, db = sum over rows of dy   (n fp32; each may be NULL).
+ * x (x_dtype) is the saved input, or NULL with codes and scales: its 8-bit rows.
+ * dy has element type y_dtype.  dx must not overlap the inputs.  rows == 0 gives
+ * zero dw and db.  The sums over rows have a fixed order.
+ */
+IFK_API int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const void* x, int64_t ld_x,
+                                   int x_dtype, const int8_t* codes, int64_t ld_codes,
+                                   const uint8_t* scales, int64_t ld_scales, const float* mean,
+                                   const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n,
+                                   void* dx, int64_t ld_dx, float* dw, float* db, void* workspace,
+                                   size_t workspace_bytes, ifk_stream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -1,0 +1,193 @@
+"""8-bit rows and layer norm on the host: the format, the checks of arguments, the
+conversion of a model.  Nothing here runs on a GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+from ifkfac_b200 import _lib
+from ifkfac_b200 import checkpoint8 as c8
+from tests import q8_reference as ref
+
+FAKE = ctypes.c_void_p(4096)
+
+
+def test_format_bounds():
+    """The oracle's format keeps what include/ifk.h promises: |x - value| <= 2^e <= a / 64."""
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((64, 100)) * np.exp(rng.uniform(-40, 40, (64, 1)))
+    x[3] = 0
+    codes, scales = ref.quantize(x)
+    v = ref.values(codes, scales, 100)
+    step = np.repeat(np.exp2(scales.astype(float) - 127), 32, axis=1)[:, :100]
+    assert (np.abs(x - v) <= step).all()
+    a = np.abs(np.pad(x, ((0, 0), (0, 28)))).reshape(64, 4, 32).max(-1)
+    assert (np.exp2(scales.astype(float) - 127)[a > 0] <= a[a > 0] / 64).all()
+    assert codes.shape == (64, 128) and (codes[:, 100:] == 0).all()
+
+
+@pytest.mark.parametrize("n,pitch", [(1, 32), (31, 32), (32, 32), (33, 64), (4096, 4096), (4097, 4128)])
+def test_pitch(n, pitch):
+    assert _lib.lib().ifk_q8_pitch(n) == pitch
+    assert _lib.lib().ifk_q8_pitch(0) == 0
+
+
+def test_q8_argument_errors_before_any_gpu_work():
+    L = _lib.lib()
+
+    def quant(x=FAKE, ld=64, dt=_lib.BF16, idx=None, src=8, rows=8, n=64, codes=FAKE, ldc=64, scales=FAKE, lds=2):
+        return L.ifk_q8_quantize(x, ld, dt, idx, src, rows, n, codes, ldc, scales, lds, None, None)
+
+    assert quant(rows=-1) == _lib.ERR_SHAPE
+    assert quant(n=0) == _lib.ERR_SHAPE
+    assert quant(ld=63) == _lib.ERR_SHAPE
+    assert quant(dt=2) == _lib.ERR_DTYPE
+    assert quant(x=None) == _lib.ERR_ARG
+    assert quant(codes=None) == _lib.ERR_ARG
+    assert quant(codes=ctypes.c_void_p(4100)) == _lib.ERR_ARG       # codes are 16-byte aligned
+    assert quant(n=65, ld=80) == _lib.ERR_SHAPE                     # the pitch of 65 columns is 96
+    assert quant(ldc=72) == _lib.ERR_SHAPE                          # not a multiple of 16
+    assert quant(lds=1) == _lib.ERR_SHAPE
+    assert quant(idx=FAKE, src=0) == _lib.ERR_SHAPE
+    assert quant(rows=0, x=None, codes=None) == _lib.OK             # nothing to do
+
+    def deq(codes=FAKE, ldc=64, scales=FAKE, lds=2, idx=None, src=8, rows=8, n=64, out=FAKE, ld=64, dt=_lib.F32):
+        return L.ifk_q8_dequantize(codes, ldc, scales, lds, idx, src, rows, n, out, ld, dt, None, None)
+
+    assert deq(out=None) == _lib.ERR_ARG
+    assert deq(scales=None) == _lib.ERR_ARG
+    assert deq(ld=63) == _lib.ERR_SHAPE
+    assert deq(ldc=32) == _lib.ERR_SHAPE
+    assert deq(dt=3) == _lib.ERR_DTYPE
+    assert deq(idx=FAKE, src=-1) == _lib.ERR_SHAPE
+    assert deq(rows=0, out=None) == _lib.OK
+
+
+def test_wgrad_argument_errors_before_any_gpu_work():
+    L = _lib.lib()
+    need = L.ifk_q8_wgrad_workspace(8, 16, 64, _lib.BF16)
+    assert need > 0
+    assert L.ifk_q8_wgrad_workspace(8, 0, 64, _lib.BF16) == 0
+    assert L.ifk_q8_wgrad_workspace(-1, 16, 64, _lib.BF16) == 0
+    assert L.ifk_q8_wgrad_workspace(8, 16, 64, 7) == 0
+
+    def wgrad(delta=FAKE, ld=16, dt=_lib.BF16, codes=FAKE, ldc=64, scales=FAKE, lds=2, rows=8, n_out=16, n_in=64,
+              dW=FAKE, ldw=64, ws=FAKE, wsb=need):
+        return L.ifk_q8_wgrad(delta, ld, dt, codes, ldc, scales, lds, rows, n_out, n_in, dW, ldw, None, 0, None, ws,
+                              wsb, None)
+
+    assert wgrad(dW=None) == _lib.ERR_ARG
+    assert wgrad(delta=None) == _lib.ERR_ARG
+    assert wgrad(codes=None) == _lib.ERR_ARG
+    assert wgrad(dt=5) == _lib.ERR_DTYPE
+    assert wgrad(rows=-1) == _lib.ERR_SHAPE
+    assert wgrad(n_out=0) == _lib.ERR_SHAPE
+    assert wgrad(n_in=0) == _lib.ERR_SHAPE
+    assert wgrad(ld=15) == _lib.ERR_SHAPE
+    assert wgrad(ldw=63) == _lib.ERR_SHAPE
+    assert wgrad(ldc=48) == _lib.ERR_SHAPE
+    assert wgrad(ws=None) == _lib.ERR_WORKSPACE
+    assert wgrad(ws=ctypes.c_void_p(4097)) == _lib.ERR_WORKSPACE
+    assert wgrad(wsb=need - 1) == _lib.ERR_WORKSPACE
+
+
+def test_layernorm_argument_errors_before_any_gpu_work():
+    L = _lib.lib()
+
+    def fwd(x=FAKE, ldx=64, xd=_lib.F32, w=FAKE, b=FAKE, wd=_lib.F32, rows=4, n=64, eps=1e-5, y=FAKE, ldy=64,
+            yd=_lib.BF16, codes=None, ldc=64, scales=None, lds=2):
+        return L.ifk_layernorm(x, ldx, xd, w, b, wd, rows, n, eps, y, ldy, yd, None, None, codes, ldc, scales, lds,
+                               None)
+
+    assert fwd(x=None) == _lib.ERR_ARG
+    assert fwd(y=None) == _lib.ERR_ARG
+    assert fwd(codes=FAKE) == _lib.ERR_ARG                  # codes without scales
+    assert fwd(codes=FAKE, scales=FAKE, ldc=32) == _lib.ERR_SHAPE
+    assert fwd(n=0) == _lib.ERR_SHAPE
+    assert fwd(rows=-1) == _lib.ERR_SHAPE
+    assert fwd(ldx=63) == _lib.ERR_SHAPE
+    assert fwd(ldy=63) == _lib.ERR_SHAPE
+    assert fwd(xd=2) == _lib.ERR_DTYPE
+    assert fwd(wd=2) == _lib.ERR_DTYPE
+    assert fwd(eps=-1e-5) == _lib.ERR_ARG
+    assert fwd(eps=float("nan")) == _lib.ERR_ARG
+    assert fwd(rows=0, x=None, y=None) == _lib.OK
+
+    need = L.ifk_layernorm_backward_workspace(4, 64)
+    assert need > 0 and L.ifk_layernorm_backward_workspace(4, 0) == 0
+
+    def bwd(dy=FAKE, ldy=64, yd=_lib.F32, x=FAKE, ldx=64, xd=_lib.F32, codes=None, scales=None, mean=FAKE, w=FAKE,
+            wd=_lib.F32, dx=FAKE, lddx=64, dw=FAKE, ws=FAKE, wsb=need):
+        return L.ifk_layernorm_backward(dy, ldy, yd, x, ldx, xd, codes, 64, scales, 2, mean, FAKE, w, wd, 4, 64, dx,
+                                        lddx, dw, None, ws, wsb, None)
+
+    assert bwd(dy=None) == _lib.ERR_ARG
+    assert bwd(mean=None) == _lib.ERR_ARG
+    assert bwd(dx=None) == _lib.ERR_ARG
+    assert bwd(x=None) == _lib.ERR_ARG                      # neither the rows nor their 8-bit form
+    assert bwd(codes=FAKE, scales=FAKE) == _lib.ERR_ARG     # both
+    assert bwd(x=None, codes=FAKE) == _lib.ERR_ARG          # codes without scales
+    assert bwd(ldy=63) == _lib.ERR_SHAPE
+    assert bwd(ldx=63) == _lib.ERR_SHAPE
+    assert bwd(lddx=63) == _lib.ERR_SHAPE
+    assert bwd(xd=9) == _lib.ERR_DTYPE
+    assert bwd(ws=None) == _lib.ERR_WORKSPACE
+    assert bwd(wsb=need - 1) == _lib.ERR_WORKSPACE
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 64)
+    q = c8.Q8Rows(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4, 2, dtype=torch.uint8), 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.quantize_rows(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.dequantize_rows(q)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.weight_grad(x, q)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.layer_norm_forward(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.LayerNorm8(64)(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        c8.Linear8(64, 8)(x)
+
+
+def test_q8rows_checks_its_layout():
+    z = lambda *s: torch.zeros(*s, dtype=torch.int8)
+    u = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+    q = c8.Q8Rows(z(6, 96), u(6, 3), 70)
+    assert (q.rows, q.cols, q.nbytes) == (6, 70, 6 * 99)
+    assert q[2:5].rows == 3 and q[2:5].codes.data_ptr() == q.codes[2].data_ptr()
+    with pytest.raises(TypeError):
+        q[::2]
+    for codes, scales, cols in ((z(6, 70), u(6, 3), 70), (z(6, 96), u(6, 2), 70), (z(6, 96), u(5, 3), 70),
+                                (z(6, 96), u(6, 3), 64), (z(6, 96), u(6, 3), 0),
+                                (z(96, 6).t(), u(6, 3), 70)):
+        with pytest.raises(ValueError):
+            c8.Q8Rows(codes, scales, cols)
+    with pytest.raises(TypeError):
+        c8.Q8Rows(u(6, 96), u(6, 3), 70)
+
+
+def test_convert_keeps_parameters_and_structure():
+    lin = nn.Linear(8, 8)
+    model = nn.Sequential(nn.LayerNorm(8), lin, nn.GELU(), lin, nn.Linear(8, 3, bias=False),
+                          nn.LayerNorm((4, 8)), nn.LayerNorm(3, elementwise_affine=False))
+    names = dict(model.named_parameters())
+    out = c8.convert(model)
+    assert out is model and dict(model.named_parameters()) == names
+    assert type(model[0]) is c8.LayerNorm8 and type(model[1]) is c8.Linear8 and type(model[4]) is c8.Linear8
+    assert model[1] is model[3]                              # a shared layer stays shared
+    assert type(model[5]) is nn.LayerNorm                    # two normalised dimensions: left alone
+    assert type(model[6]) is c8.LayerNorm8 and model[6].weight is None
+    assert model[1].weight is lin.weight and model[4].bias is None and model[0].eps == 1e-5
+    hooked = nn.Sequential(nn.Linear(4, 4))
+    hooked[0].register_forward_hook(lambda *a: None)
+    assert type(c8.convert(hooked)[0]) is nn.Linear          # its hooks would be lost
+    only = c8.convert(nn.Sequential(nn.Linear(4, 4), nn.LayerNorm(4)), linear=False)
+    assert type(only[0]) is nn.Linear and type(only[1]) is c8.LayerNorm8
+    assert type(c8.convert(nn.Linear(4, 4))) is c8.Linear8
+    with pytest.raises(ValueError):
+        c8.LayerNorm8((4, 8))
