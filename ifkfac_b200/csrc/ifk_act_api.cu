@@ -15,6 +15,8 @@ bool aligned(const void* p) { return ((uintptr_t)p % ALIGN) == 0; }
 bool dtype_ok(int d) { return d == IFK_F32 || d == IFK_BF16; }
 cudaStream_t S(ifk_stream_t s) { return (cudaStream_t)s; }
 
+constexpr int64_t MAX_SIDE = 1 << 28;
+
 // Layout of 8-bit rows of n columns.
 int q8_rows_ok(const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t n) {
   if (!codes || !scales || ((uintptr_t)codes & 15)) return IFK_ERR_ARG;
@@ -58,6 +60,7 @@ int ifk_q8_dequantize(const int8_t* codes, int64_t ld_codes, const uint8_t* scal
 
 size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in, int delta_dtype) {
   if (rows < 0 || n_out <= 0 || n_in <= 0 || !dtype_ok(delta_dtype)) return 0;
+  if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return 0;
   return align_up(q8_wgrad_bytes(rows, n_out, n_in, delta_dtype)) + ALIGN;
 }
 
@@ -67,6 +70,7 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
                  ifk_stream_t stream) {
   if (!dW) return IFK_ERR_ARG;
   if (rows < 0 || n_out <= 0 || n_in <= 0 || ld_dW < n_in) return IFK_ERR_SHAPE;
+  if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return IFK_ERR_SHAPE;  // 32-bit tile coordinates
   if (!dtype_ok(delta_dtype)) return IFK_ERR_DTYPE;
   cudaStream_t s = S(stream);
   if (rows == 0) {
