@@ -7,15 +7,13 @@
 // columns), so the accumulator in TMEM has an input column a lane and the
 // epilogue's stores are contiguous along dW's rows.
 //
-// Per step of 64 rows, TMA brings delta (bf16, 128-byte swizzle) and the codes
-// into a stage; eight warps turn the codes into bf16 in the same layout; one
-// thread issues the four tcgen05.mma of the step.  A code times its power-of-two
-// scale is exact in bf16, so the products are exact and only the fp32 sums round.
-// An fp32 delta is taken apart beforehand into three bf16 terms (8 + 8 + 8 bits,
-// by truncation: exact), and each 64 rows take three steps.
-//
-// With CG = 2 a pair of CTAs shares one 256 x 256 tile (tcgen05 cta_group::2): each
-// converts its own 128 input columns and loads half of delta's columns.
+// A pair of CTAs shares one 256 x 256 tile (tcgen05 cta_group::2).  Per step of 64
+// rows each CTA brings half of delta's columns (bf16) and its own 128 columns of codes
+// by TMA, four warps turn the codes into a bf16 tile, and one thread of the pair issues
+// the step's four tcgen05.mma.  A code times its power-of-two scale is exact in bf16,
+// so the products are exact and only the fp32 sums round.  An fp32 delta is taken apart
+// beforehand into three bf16 terms (8 + 8 + 8 bits, by truncation: exact), and each 64
+// rows take three steps.
 //
 // The tensor core truncates as it adds to the accumulator, so a long sum drifts
 // towards zero by about 7e-9 of itself a tcgen05.mma; after CHUNK steps (120 of them)
@@ -41,23 +39,29 @@ constexpr int KS = 64;        // rows a step
 constexpr int TM = 128;       // input columns a CTA
 constexpr int TN = 256;       // output columns a tile
 constexpr int CHUNK = 30;     // steps a TMEM accumulator sums: 30 row blocks, or 10 in three terms
-constexpr int CONV_WARPS = 4; // a step's converting warps; two such groups take turns
-constexpr int THREADS = 512;  // warps: 0 TMA, 1 MMA, 2 TMEM, 3 scales, 4-7 epilogue, 8-15 conversion
-constexpr int AHEAD = 4;      // steps the scales are loaded ahead
-constexpr uint32_t A_BYTES = TM * KS * 2, C_BYTES = TM * KS;
-constexpr uint32_t ATOM = 64 * KS * 2;  // 64 columns (128 bytes) of KS rows
-constexpr int SM_COUNT = 148;
+constexpr int CONV_WARPS = 4;   // converting warps of a step
+constexpr int CONV_GROUPS = 4;  // such groups, taking turns
+// warps: 0 delta, 1 MMA, 2 TMEM and codes, 3 scales, 4-7 epilogue, 8 .. conversion
+constexpr int THREADS = 32 * (8 + CONV_WARPS * CONV_GROUPS);
+constexpr int SM_COUNT = 148, CLUSTERS = SM_COUNT / 2;
 constexpr int MIN_STEPS = 4;  // least steps a share of a cut tile is worth
+constexpr uint32_t ATOM = 64 * KS * 2;  // 64 columns (128 bytes) of KS rows
 
-template <int CG>
-struct Cfg {
-  static constexpr uint32_t B_BYTES = TN / CG * KS * 2;
-  static constexpr uint32_t STAGE = A_BYTES + B_BYTES + C_BYTES;
-  static constexpr int STAGES = CG == 2 ? 5 : 4;
-  static constexpr uint32_t SCALES = STAGES * STAGE;  // per stage KS x 4 bytes
-  static constexpr uint32_t BARS = SCALES + STAGES * KS * 4;
-  static constexpr uint32_t SMEM = BARS + (3 * STAGES + 4) * 8 + 16;
-};
+// Shared memory: a ring of NS steps (a converted tile and delta's half each), a ring of
+// NC steps of codes and scales, the barriers.  A load takes about a microsecond, a step at
+// the tensor core's rate a third of one.
+constexpr int NS = 6, NC = 4;
+// A parity wait also passes one phase early, so whoever waits on a barrier has to have seen
+// the phase before.  A converting group's slots of codes are its own; and before it writes
+// a tile, step i waits for the products of step i - NS, of which the phase before is step
+// i - 2 NS, while the group's last step has waited for step i - NS - CONV_GROUPS.
+static_assert(NC == CONV_GROUPS && CONV_GROUPS <= NS, "rings and groups");
+constexpr uint32_t A_BYTES = TM * KS * 2, D_BYTES = TN / 2 * KS * 2, C_BYTES = TM * KS;
+constexpr uint32_t O_TILES = 0, O_DELTA = O_TILES + NS * A_BYTES, O_CODES = O_DELTA + NS * D_BYTES;
+constexpr uint32_t O_SCALES = O_CODES + NC * C_BYTES;  // per slot KS x 4 bytes
+constexpr uint32_t O_BARS = O_SCALES + NC * KS * 4;
+constexpr int NBARS = 2 * NC + 2 * NS + 4;
+constexpr uint32_t SMEM = O_BARS + NBARS * 8 + 16;
 
 // Division of the tiles between clusters.
 struct Plan {
@@ -78,9 +82,10 @@ struct Args {
   const uint8_t* scales;
   int64_t lds, rows, n_out, n_in, ldw;
   float* dW;
-  float* part;         // [2 Gs][TN][CG TM]
+  float* part;         // [2 Gs][TN][2 TM]
   int accumulate;
   bool vec_scales;     // rows of scales start at multiples of 4 bytes
+  bool whole;          // delta's map has 64-column blocks as a dimension (n_out a multiple of 64)
   int* status;
 };
 
@@ -105,6 +110,18 @@ struct Piece {
   int tile, k0, k1, slot;
 };
 
+// Position in a ring of N slots: the slot and the parity of its round.
+template <int N>
+struct Ring {
+  uint32_t s = 0, ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
 // The pieces of cluster c in order.
 struct Walk {
   const Plan& p;
@@ -115,6 +132,9 @@ struct Walk {
       at = p.share(c);
       end = p.share(c + 1);
     }
+  }
+  __device__ int64_t steps() const {
+    return (c < p.Tdp ? (int64_t)((p.Tdp - 1 - c) / p.G + 1) * p.Kt : 0) + (end - at);
   }
   __device__ bool next(Piece& w) {
     if (next_tile < p.Tdp) {
@@ -152,7 +172,7 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -170,32 +190,53 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
   }
 }
 
+// One arrival, and the bytes of the copies that the barrier's phase also waits for.
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done;
+}
+// The address of the same place in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// After a failed wait: stay until the copies in flight have landed (microseconds).
+__device__ __forceinline__ void linger() {
+  const uint64_t t0 = now_ns();
+  while (now_ns() - t0 < 1000000ull) __nanosleep(1000);
+}
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
           "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+// A copy into this CTA's memory that completes on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int t,
+                                            uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-      "[%5];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(t), "r"(bar)
       : "memory");
-}
-
-// Arrive on the barrier at the same offset in the cluster's first CTA.
-template <int CG>
-__device__ __forceinline__ void arrive_leader(uint32_t bar) {
-  if (CG == 1) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .b32 ra;\n\t"
-        "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
-        "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}\n" ::"r"(bar)
-        : "memory");
-  }
 }
 
 // Operand tiles: M/N-major, 128-byte swizzle.  64 columns of 8 rows are one 1024-byte
@@ -205,60 +246,26 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
          (1ull << 46) | (2ull << 61);
 }
 
-template <int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
-  if (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
-        : "memory");
+// D (+)= A B over the pair's two halves; issued by one thread of its first CTA.
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
 }
 
-// Arrive on this barrier (in both CTAs of a pair) when the MMAs issued so far are done.
-template <int CG>
-__device__ __forceinline__ void commit(uint32_t bar) {
-  if (CG == 1)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-  else
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
+// Arrive on this barrier in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
 }
 
-template <int CG>
-__device__ __forceinline__ void alloc_tmem(uint32_t slot) {
-  if (CG == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-}
-template <int CG>
-__device__ __forceinline__ void free_tmem(uint32_t base) {
-  if (CG == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
-  else
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
-}
-
-template <int CG>
-__device__ __forceinline__ void sync_cluster() {
-  if (CG == 1) {
-    __syncthreads();
-  } else {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
+__device__ __forceinline__ void sync_pair() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Four packed codes to four bf16 values, exactly.  With the byte's low seven bits under
@@ -277,36 +284,42 @@ __device__ __forceinline__ void codes4(uint32_t w, __nv_bfloat162 scale, uint32_
   hi = r[1];
 }
 
-template <int CG>
 __global__ void __launch_bounds__(THREADS, 1)
 wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ CUtensorMap cmap, const Args a) {
-  using C = Cfg<CG>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc::smem_u32(smem);
-  const uint32_t full = base + C::BARS, ready = full + 8 * C::STAGES, empty = ready + 8 * C::STAGES;
-  const uint32_t acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::BARS + (3 * C::STAGES + 4) * 8);
+  // codes_full: codes and scales have landed; codes_free: they are converted;
+  // ready (first CTA): both CTAs' tiles are converted and both halves of delta have landed;
+  // free: the step is multiplied; acc_full / acc_free: an accumulator is summed / read
+  const uint32_t codes_full = base + O_BARS, codes_free = codes_full + 8 * NC;
+  const uint32_t ready = codes_free + 8 * NC, free = ready + 8 * NS, acc_full = free + 8 * NS, acc_free = acc_full + 16;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + O_BARS + NBARS * 8);
   volatile int* failed = reinterpret_cast<volatile int*>(slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? (blockIdx.x & 1) : 0;
-  const int cluster = blockIdx.x / CG;
+  const uint32_t rank = blockIdx.x & 1;
+  const int cluster = blockIdx.x >> 1;
 
   if (threadIdx.x == 0) {
     *failed = 0;
-    for (int s = 0; s < C::STAGES; ++s) {
-      tc::mbar_init(reinterpret_cast<uint64_t*>(smem + C::BARS) + s, 2);  // the copies and the scales
-      tc::mbar_init(reinterpret_cast<uint64_t*>(smem + C::BARS) + C::STAGES + s, CONV_WARPS * CG);
-      tc::mbar_init(reinterpret_cast<uint64_t*>(smem + C::BARS) + 2 * C::STAGES + s, 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(reinterpret_cast<uint64_t*>(smem + C::BARS) + 3 * C::STAGES + b, 1);
-      tc::mbar_init(reinterpret_cast<uint64_t*>(smem + C::BARS) + 3 * C::STAGES + 2 + b, 4 * CG);
-    }
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + O_BARS);
+    auto init = [&](int count, uint32_t arrivals) {
+      for (int i = 0; i < count; ++i) tc::mbar_init(bar++, arrivals);
+    };
+    init(NC, 1 + 32);              // codes_full: the copy, and the lanes that bring the scales
+    init(NC, CONV_WARPS);          // codes_free
+    init(NS, 1 + CONV_WARPS * 2);  // ready: the copies, and both CTAs' warps
+    init(NS, 1);                   // free
+    init(2, 1);                    // acc_full
+    init(2, 4 * 2);                // acc_free
   }
-  if (warp == 2) alloc_tmem<CG>(tc::smem_u32(slot));
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::smem_u32(slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
   tc::fence_before();
   __syncthreads();
-  sync_cluster<CG>();
+  sync_pair();
   tc::fence_after();
   const uint32_t tmem = *slot;
 
@@ -314,62 +327,64 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
   Piece w;
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
+      Ring<NS> r;
+      const uint32_t bar0 = in_leader(ready);
+      bool ok = true, now = true;
       while (ok && walk.next(w)) {
-        const int ti = w.tile % a.p.Ti, to = w.tile / a.p.Ti;
-        const int x = (ti * CG + (int)rank) * TM, o = to * TN + (int)rank * (TN / CG);
-        for (int k = w.k0; k < w.k1; ++k, ++it) {
-          const uint32_t s = it % C::STAGES, ph = it / C::STAGES & 1;
-          if (!wait_bar(empty + 8 * s, ph ^ 1, failed)) {
+        const int o = w.tile / a.p.Ti * TN + (int)rank * (TN / 2);
+        for (int k = w.k0; k < w.k1; ++k) {
+          if (!now && !wait_bar(free + 8 * r.s, r.ph ^ 1, failed)) {
             ok = false;
             break;
           }
-          const uint32_t st = base + s * C::STAGE, bar = full + 8 * s;
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::B_BYTES + C_BYTES)
-                       : "memory");
           const Step sp = step_at(a, k);
-          const int row = sp.block * KS;
-          tma_2d(st + A_BYTES + C::B_BYTES, &cmap, x, row, bar);
-#pragma unroll
-          for (int j = 0; j < TN / CG / 64; ++j)
-            tma_3d(st + A_BYTES + j * ATOM, &dmap, o + j * 64, row, sp.term, bar);
+          const uint32_t dst = base + O_DELTA + r.s * D_BYTES, bar = bar0 + 8 * r.s;
+          if (rank == 0) expect(ready + 8 * r.s, 2 * D_BYTES);  // both CTAs' copies
+          if (a.whole) {
+            tma_4d_pair(dst, &dmap, 0, sp.block * KS, o >> 6, sp.term, bar);
+          } else {
+            tma_4d_pair(dst, &dmap, o, sp.block * KS, 0, sp.term, bar);
+            tma_4d_pair(dst + ATOM, &dmap, o + 64, sp.block * KS, 0, sp.term, bar);
+          }
+          r.next();
+          now = test_bar(free + 8 * r.s, r.ph ^ 1);
         }
       }
-      // leave with no copy in flight (the last STAGES steps'); after a failed wait too
-      for (uint32_t q = it > C::STAGES ? it - C::STAGES : 0; q < it; ++q) {
-        int quiet = 0;
-        if (!wait_bar(full + 8 * (q % C::STAGES), q / C::STAGES & 1, &quiet)) break;
-      }
+      if (!ok) linger();
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = tc::idesc_bf16(TM * CG, TN, true, true);
-      uint32_t it = 0, buf = 0, bph = 0;
-      bool ok = true;
+      constexpr uint32_t idesc = tc::idesc_bf16(TM * 2, TN, true, true);
+      const uint64_t ad0 = desc_sw128(base + O_TILES), bd0 = desc_sw128(base + O_DELTA);
+      Ring<NS> r;
+      uint32_t buf = 0, bph = 0;
+      bool ok = true, now = false;
       while (ok && walk.next(w)) {
         for (int c0 = w.k0, c1; ok && c0 < w.k1; c0 = c1) {
           c1 = chunk_end(c0, w.k1);
-          if (!wait_bar(acc_empty + 8 * buf, bph ^ 1, failed)) {
+          if (!wait_bar(acc_free + 8 * buf, bph ^ 1, failed)) {
             ok = false;
             break;
           }
           tc::fence_after();
-          for (int k = c0; k < c1; ++k, ++it) {
-            const uint32_t s = it % C::STAGES, ph = it / C::STAGES & 1;
-            if (!wait_bar(ready + 8 * s, ph, failed)) {
+          const uint32_t acc = tmem + buf * TN;
+          for (int k = c0; k < c1; ++k) {
+            if (!now && !wait_bar(ready + 8 * r.s, r.ph, failed)) {
               ok = false;
               break;
             }
             tc::fence_after();
-            const uint64_t ad = desc_sw128(base + s * C::STAGE), bd = desc_sw128(base + s * C::STAGE + A_BYTES);
-#pragma unroll
-            for (int j = 0; j < KS / 16; ++j)
-              mma<CG>(tmem + buf * TN, ad + tc::doff(j * 2048), bd + tc::doff(j * 2048), idesc,
-                      (k > c0 || j > 0) ? 1u : 0u);
-            commit<CG>(empty + 8 * s);
+            const uint64_t ad = ad0 + tc::doff(r.s * A_BYTES), bd = bd0 + tc::doff(r.s * D_BYTES);
+            const uint32_t bar = free + 8 * r.s;
+            r.next();
+            mma_pair(acc, ad, bd, idesc, k > c0 ? 1u : 0u);
+            mma_pair(acc, ad + tc::doff(2048), bd + tc::doff(2048), idesc, 1u);
+            now = test_bar(ready + 8 * r.s, r.ph);  // the next step's, while this one's products are issued
+            mma_pair(acc, ad + tc::doff(2 * 2048), bd + tc::doff(2 * 2048), idesc, 1u);
+            mma_pair(acc, ad + tc::doff(3 * 2048), bd + tc::doff(3 * 2048), idesc, 1u);
+            commit_pair(bar);
           }
-          commit<CG>(acc_full + 8 * buf);
+          commit_pair(acc_full + 8 * buf);
           if (!ok) {
             // a wait gave up: leave once the products already issued are done
             int quiet = 0;
@@ -380,52 +395,61 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
         }
       }
     }
-  } else if (warp == 3) {
-    // the scale bytes of a stage: rows lane and lane + 32, four groups each, loaded AHEAD steps early
-    uint32_t it = 0;
-    bool ok = true;
-    const int64_t groups = q8::pitch(a.n_in) / q8::GROUP;
-    while (ok && walk.next(w)) {
-      const int64_t gi = (int64_t)(w.tile % a.p.Ti * CG + (int)rank) * (TM / q8::GROUP);
-      const bool vec = a.vec_scales && gi + 4 <= groups;
-      auto load = [&](int k, int h) -> uint32_t {
-        if (k >= w.k1) return 0u;
-        const int64_t r = (int64_t)step_at(a, k).block * KS + h * 32 + lane;
-        if (r >= a.rows) return 0u;
-        const uint8_t* p = a.scales + r * a.lds + gi;
-        if (vec) return *reinterpret_cast<const uint32_t*>(p);
-        uint32_t v = 0;
-        for (int g = 0; g < 4; ++g)
-          if (gi + g < groups) v |= (uint32_t)p[g] << (8 * g);
-        return v;
-      };
-      uint32_t q[AHEAD][2];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        q[j][0] = load(w.k0 + j, 0);
-        q[j][1] = load(w.k0 + j, 1);
-      }
-      for (int k = w.k0; ok && k < w.k1; k += AHEAD) {
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          if (!ok || k + j >= w.k1) break;
-          const uint32_t s = it % C::STAGES, ph = it / C::STAGES & 1;
-          if (!wait_bar(empty + 8 * s, ph ^ 1, failed)) {
+  } else if (warp == 2) {
+    if (lane == 0) {
+      Ring<NC> r;
+      bool ok = true, now = true;
+      while (ok && walk.next(w)) {
+        const int x = (w.tile % a.p.Ti * 2 + (int)rank) * TM;
+        for (int k = w.k0; k < w.k1; ++k) {
+          if (!now && !wait_bar(codes_free + 8 * r.s, r.ph ^ 1, failed)) {
             ok = false;
             break;
           }
-          uint32_t* d = reinterpret_cast<uint32_t*>(smem + C::SCALES + s * (KS * 4));
-          d[lane] = q[j][0];
-          d[32 + lane] = q[j][1];
-          q[j][0] = load(k + j + AHEAD, 0);
-          q[j][1] = load(k + j + AHEAD, 1);
-          __syncwarp();
-          if (lane == 0)
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + 8 * s) : "memory");
-          ++it;
+          expect(codes_full + 8 * r.s, C_BYTES);
+          tma_2d(base + O_CODES + r.s * C_BYTES, &cmap, x, step_at(a, k).block * KS, codes_full + 8 * r.s);
+          r.next();
+          now = test_bar(codes_free + 8 * r.s, r.ph ^ 1);
         }
       }
+      if (!ok) linger();
     }
+  } else if (warp == 3) {
+    // the scale bytes of a slot: rows lane and lane + 32, four groups each; a row past the end has zeros
+    Ring<NC> r;
+    bool ok = true;
+    const int64_t groups = q8::pitch(a.n_in) / q8::GROUP;
+    while (ok && walk.next(w)) {
+      const int64_t gi = (int64_t)(w.tile % a.p.Ti * 2 + (int)rank) * (TM / q8::GROUP);
+      const bool vec = a.vec_scales && gi + 4 <= groups;
+      for (int k = w.k0; k < w.k1; ++k, r.next()) {
+        if (!wait_bar(codes_free + 8 * r.s, r.ph ^ 1, failed)) {
+          ok = false;
+          break;
+        }
+        const int64_t row0 = (int64_t)step_at(a, k).block * KS;
+        const uint32_t bar = codes_full + 8 * r.s;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t row = row0 + h * 32 + lane;
+          const uint32_t off = O_SCALES + r.s * (KS * 4) + (h * 32 + lane) * 4;
+          const bool in = row < a.rows;
+          const uint8_t* p = a.scales + (in ? row : 0) * a.lds + (vec ? gi : 0);
+          if (vec) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + off), "l"(p), "r"(in ? 4 : 0)
+                         : "memory");
+          } else {
+            uint32_t v = 0;
+            for (int g = 0; g < 4; ++g)
+              if (in && gi + g < groups) v |= (uint32_t)p[gi + g] << (8 * g);
+            *reinterpret_cast<uint32_t*>(smem + off) = v;
+          }
+        }
+        if (vec) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+        else arrive(bar);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= 4 && warp < 8) {
     uint32_t buf = 0, bph = 0;
     const int wq = warp & 3;  // the quarter of TMEM's lanes this warp reads
@@ -433,11 +457,11 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
     while (ok && walk.next(w)) {
       const int ti = w.tile % a.p.Ti, to = w.tile / a.p.Ti;
       const int m = (int)rank * TM + wq * 32 + lane;
-      const int64_t i = (int64_t)ti * CG * TM + m, o0 = (int64_t)to * TN;
+      const int64_t i = (int64_t)ti * 2 * TM + m, o0 = (int64_t)to * TN;
       // where this thread's column of the tile goes: dW, or its share's slot
       const bool to_part = w.slot >= 0;
-      float* d = to_part ? a.part + (int64_t)w.slot * (TN * CG * TM) + m : a.dW + o0 * a.ldw + i;
-      const int64_t ld = to_part ? CG * TM : a.ldw;
+      float* d = to_part ? a.part + (int64_t)w.slot * (TN * 2 * TM) + m : a.dW + o0 * a.ldw + i;
+      const int64_t ld = to_part ? 2 * TM : a.ldw;
       const int cols = to_part ? TN : (i < a.n_in ? (int)mn<int64_t>(TN, a.n_out - o0) : 0);
       bool add = !to_part && a.accumulate;
       for (int c0 = w.k0; c0 < w.k1; c0 = chunk_end(c0, w.k1)) {
@@ -470,82 +494,90 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
         add = true;
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) arrive_leader<CG>(acc_empty + 8 * buf);
+        if (lane == 0) arrive_cluster(in_leader(acc_free + 8 * buf));
         buf ^= 1;
         if (buf == 0) bph ^= 1;
       }
     }
-  } else if (warp >= 8) {
-    // this thread's group of 32 columns and its two rows of every other step
+  } else {
+    // this thread's group of 32 columns, and its rows of every CONV_GROUPS-th step
+    constexpr int RPT = KS / 8 / CONV_WARPS;
     const int grp = (warp - 8) / CONV_WARPS, r0 = (warp - 8) % CONV_WARPS * 8 + (lane & 7), g = lane >> 3;
-    uint32_t it = 0;
-    bool ok = true;
-    while (ok && walk.next(w)) {
-      const uint32_t end = it + (uint32_t)(w.k1 - w.k0);
-      for (; it < end; ++it) {
-        if ((int)(it & 1) != grp) continue;
-        const uint32_t s = it % C::STAGES, ph = it / C::STAGES & 1;
-        if (!wait_bar(full + 8 * s, ph, failed)) {
-          ok = false;
-          break;
-        }
-        const uint32_t st = base + s * C::STAGE;
+    const int64_t steps = walk.steps();
+    const uint32_t full = codes_full + 8 * grp, src0 = base + O_CODES + grp * C_BYTES;
+    const uint8_t* sc0 = smem + O_SCALES + grp * (KS * 4) + g;
+    const uint32_t ready0 = in_leader(ready);
+    uint32_t cph = 0, s = grp, ph = 0;  // phase of the codes' slot; slot of the step and its phase
+    for (int64_t i = grp; i < steps; i += CONV_GROUPS) {
+      if (!wait_bar(full, cph, failed)) break;
+      cph ^= 1;
+      // every read in flight before the first conversion
+      uint32_t cw[RPT][2][4], sb[RPT], o[RPT][4][4];
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const int kr = r0 + rr * 32;
-          const uint32_t src = st + A_BYTES + C::B_BYTES + kr * 128;
-          const uint32_t dst = st + (g >> 1) * ATOM + kr * 128;
-          const uint32_t s0 = smem[C::SCALES + s * (KS * 4) + kr * 4 + g];
-          const uint32_t sb = s0 << 7 | s0 << 23;  // 2^e as bf16, twice (byte 255: infinity)
-          const __nv_bfloat162 sc = *reinterpret_cast<const __nv_bfloat162*>(&sb);
+      for (int rr = 0; rr < RPT; ++rr) {
+        const int kr = r0 + rr * 8 * CONV_WARPS;
+        sb[rr] = sc0[kr * 4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t cw[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(cw[0]), "=r"(cw[1]), "=r"(cw[2]), "=r"(cw[3])
-                         : "r"(src + (((2 * g + h) ^ (kr & 7)) << 4)));
+        for (int h = 0; h < 2; ++h)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(cw[rr][h][0]), "=r"(cw[rr][h][1]), "=r"(cw[rr][h][2]), "=r"(cw[rr][h][3])
+                       : "r"(src0 + kr * 128 + (((2 * g + h) ^ (kr & 7)) << 4)));
+      }
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t o[4];
-              codes4(cw[2 * q], sc, o[0], o[1]);
-              codes4(cw[2 * q + 1], sc, o[2], o[3]);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                               dst + ((((g & 1) * 4 + h * 2 + q) ^ (kr & 7)) << 4)),
-                           "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
-                           : "memory");
-            }
-          }
-        }
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(ready + 8 * s);
+      for (int rr = 0; rr < RPT; ++rr) {
+        const uint32_t s2 = sb[rr] << 7 | sb[rr] << 23;  // 2^e as bf16, twice (byte 255: infinity)
+        const __nv_bfloat162 sc = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          codes4(cw[rr][q >> 2][q & 3], sc, o[rr][q >> 1][(q & 1) * 2], o[rr][q >> 1][(q & 1) * 2 + 1]);
+      }
+      __syncwarp();
+      if (lane == 0) arrive(codes_free + 8 * grp);
+      if (!wait_bar(free + 8 * s, ph ^ 1, failed)) break;
+#pragma unroll
+      for (int rr = 0; rr < RPT; ++rr) {
+        const int kr = r0 + rr * 8 * CONV_WARPS;
+        const uint32_t dst = base + O_TILES + s * A_BYTES + (g >> 1) * ATOM + kr * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((((g & 1) * 4 + q) ^ (kr & 7)) << 4)),
+                       "r"(o[rr][q][0]), "r"(o[rr][q][1]), "r"(o[rr][q][2]), "r"(o[rr][q][3])
+                       : "memory");
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(ready0 + 8 * s);
+      s += CONV_GROUPS;
+      if (s >= NS) {
+        s -= NS;
+        ph ^= 1;
       }
     }
   }
   __syncwarp();
   __syncthreads();
-  sync_cluster<CG>();
+  sync_pair();
   if (threadIdx.x == 0 && *failed && a.status) *a.status = IFK_ERR_TIMEOUT;
-  if (warp == 2) free_tmem<CG>(tmem);
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // A cut tile's shares, added in the order of the rows.  A block takes 16 output columns.
-template <int CG>
-__global__ void __launch_bounds__(CG * TM) join_kernel(const Args a) {
+__global__ void __launch_bounds__(2 * TM) join_kernel(const Args a) {
   const Plan& p = a.p;
   const int64_t t = blockIdx.x, b = t * p.Kt;
   const int w0 = p.owner(b), w1 = p.owner(b + p.Kt - 1);
   if (w0 == w1) return;  // one cluster had it all
   const int tile = p.Tdp + (int)t;
-  const int64_t i = (int64_t)(tile % p.Ti) * CG * TM + threadIdx.x;
+  const int64_t i = (int64_t)(tile % p.Ti) * 2 * TM + threadIdx.x;
   const int64_t o0 = (int64_t)(tile / p.Ti) * TN + blockIdx.y * 16;
   if (i >= a.n_in) return;
-  constexpr int64_t SLOT = TN * CG * TM;
-  const float* src = a.part + (int64_t)blockIdx.y * 16 * (CG * TM) + threadIdx.x;
+  constexpr int64_t SLOT = TN * 2 * TM;
+  const float* src = a.part + (int64_t)blockIdx.y * 16 * (2 * TM) + threadIdx.x;
 #pragma unroll 4
   for (int q = 0; q < 16; ++q) {
     if (o0 + q >= a.n_out) break;
-    const float* s = src + q * (CG * TM);
+    const float* s = src + q * (2 * TM);
     float v = s[(2 * w0 + 1) * SLOT];
     for (int c = w0 + 1; c <= w1; ++c) v += s[2 * c * SLOT];
     float* d = a.dW + (o0 + q) * a.ldw + i;
@@ -636,15 +668,13 @@ struct Layout {
   size_t sums, terms_b, part;
 };
 
-constexpr int CG_USED = 2;
-
 Plan make_plan(int64_t rows, int64_t n_out, int64_t n_in, int terms) {
   Plan p;
-  p.Ti = (int)cdiv(n_in, TM * CG_USED);
+  p.Ti = (int)cdiv(n_in, TM * 2);
   p.To = (int)cdiv(n_out, TN);
   p.Kt = (int)cdiv(rows, KS) * terms;
   const int64_t T = (int64_t)p.Ti * p.To;
-  const int most = SM_COUNT / CG_USED;
+  const int most = CLUSTERS;
   p.Tdp = (int)(T / most * most);
   p.total = (T - p.Tdp) * p.Kt;
   // shares of at least MIN_STEPS steps, or of whole tiles
@@ -661,7 +691,7 @@ Layout layout(int64_t rows, int64_t n_out, int64_t n_in, int dtype, bool copy) {
   l.sums = up256((size_t)sum_splits(rows, n_out) * (size_t)n_out * sizeof(float));
   l.terms_b = l.copy ? up256((size_t)l.terms * (size_t)rows * (size_t)l.ldo * 2) : 0;
   const Plan p = make_plan(rows, n_out, n_in, l.terms);
-  l.part = p.total ? (size_t)2 * p.Gs * TN * CG_USED * TM * sizeof(float) : 0;
+  l.part = p.total ? (size_t)2 * p.Gs * TN * 2 * TM * sizeof(float) : 0;
   return l;
 }
 
@@ -680,12 +710,16 @@ EncodeFn encoder() {
   return fn;
 }
 
-// delta's terms: columns, rows, terms; boxes of 64 columns (128 bytes) x KS rows.
-bool delta_map(CUtensorMap* m, const void* d, int64_t ld, int64_t rows, int64_t n, int terms) {
-  const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)rows, (cuuint64_t)terms};
-  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows};
-  const cuuint32_t box[3] = {64, KS, 1}, one[3] = {1, 1, 1};
-  return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(d), dims, strides, box, one,
+// delta's terms in boxes of 64 columns (128 bytes) x KS rows.  whole: blocks of 64 columns
+// are a dimension of their own, and a box has the two that a CTA takes; otherwise (a ragged
+// last block) a box has one, and columns past n read as 0.
+bool delta_map(CUtensorMap* m, const void* d, int64_t ld, int64_t rows, int64_t n, int terms, bool whole) {
+  const cuuint64_t pitch = (cuuint64_t)ld * 2;
+  const cuuint64_t dims[4] = {whole ? 64 : (cuuint64_t)n, (cuuint64_t)rows, whole ? (cuuint64_t)n / 64 : 1,
+                              (cuuint64_t)terms};
+  const cuuint64_t strides[3] = {pitch, whole ? 128 : pitch * (cuuint64_t)rows, pitch * (cuuint64_t)rows};
+  const cuuint32_t box[4] = {64, KS, whole ? 2u : 1u, 1}, one[4] = {1, 1, 1, 1};
+  return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(d), dims, strides, box, one,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -698,29 +732,27 @@ bool codes_map(CUtensorMap* m, const int8_t* c, int64_t ld, int64_t rows, int64_
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int CG>
 int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, cudaStream_t s) {
   static thread_local int done_dev = -1;
   int dev = 0;
   IFK_CUDA_TRY(cudaGetDevice(&dev));
   if (done_dev != dev) {
-    IFK_CUDA_TRY(cudaFuncSetAttribute(wgrad_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)Cfg<CG>::SMEM));
+    IFK_CUDA_TRY(cudaFuncSetAttribute(wgrad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     done_dev = dev;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.p.G * CG));
+  cfg.gridDim = dim3((unsigned)(a.p.G * 2));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Cfg<CG>::SMEM;
+  cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.x = 2;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel<CG>, dm, cm, a));
-  if (a.p.total) join_kernel<CG><<<dim3((unsigned)(a.p.total / a.p.Kt), TN / 16), CG * TM, 0, s>>>(a);
+  IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel, dm, cm, a));
+  if (a.p.total) join_kernel<<<dim3((unsigned)(a.p.total / a.p.Kt), TN / 16), 2 * TM, 0, s>>>(a);
   IFK_CUDA_TRY(cudaGetLastError());
   return IFK_OK;
 }
@@ -759,8 +791,10 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
     ld = l.ldo;
   }
   CUtensorMap dm, cm;
-  if (!delta_map(&dm, src, ld, rows, n_out, l.terms) || !codes_map(&cm, codes, ldc, rows, n_in)) return IFK_ERR_SHAPE;
-  const int rc = launch<CG_USED>(dm, cm, a, s);
+  a.whole = n_out % 64 == 0;
+  if (!delta_map(&dm, src, ld, rows, n_out, l.terms, a.whole) || !codes_map(&cm, codes, ldc, rows, n_in))
+    return IFK_ERR_SHAPE;
+  const int rc = launch(dm, cm, a, s);
   if (rc != IFK_OK || !db) return rc;
   const int64_t parts = sum_splits(rows, n_out);
   column_sums_kernel<TD><<<dim3((unsigned)cdiv(n_out, 256), (unsigned)parts), 256, 0, s>>>(
