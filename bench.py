@@ -843,10 +843,14 @@ def run_c4(args, rank, world, local_rank):
     bf16 autocast, K-FAC on every Linear of the blocks (qkv 768->2304, proj, fc 768->3072,
     fc2 3072->768; the 50257-wide head excluded by max_out_dim = 4096), use_true_bf16,
     damping 1e-3, every token's rows (max_seq_rows = 0), batched_qr, momentum 0.9,
-    factor_update_freq 10.  A step is forward + backward + IFKFAC.step."""
+    factor_update_freq 10.  A step is forward + backward + IFKFAC.step.
+
+    ``--act8`` holds the activations in 8 bits: Linear8 / LayerNorm8 in place of the
+    Linear and LayerNorm layers, and capture_8bit."""
     import torch
     import torch.nn as nn
     import torch.nn.functional as F
+    from ifkfac_b200.checkpoint8 import convert
     from ifkfac_b200.ifkfac import IFKFAC
     torch.cuda.set_device(local_rank)
     dev = torch.device("cuda", local_rank)
@@ -882,11 +886,13 @@ def run_c4(args, rank, world, local_rank):
 
     torch.manual_seed(0)
     model = GPT().to(dev)
+    if args.act8:
+        convert(model)
     g = torch.Generator(device=dev).manual_seed(0)
     idx = torch.randint(0, vocab, (batch, seq + 1), generator=g, device=dev)
     x, y = idx[:, :-1], idx[:, 1:]
     opt = IFKFAC(model, lr=1e-3, damping=1e-3, factor_update_freq=10, momentum=0.9, use_true_bf16=True,
-                 max_out_dim=4096, max_seq_rows=0, batched_qr=True)
+                 max_out_dim=4096, max_seq_rows=0, batched_qr=True, capture_8bit=args.act8)
 
     def one():
         opt.zero_grad()
@@ -915,8 +921,10 @@ def run_c4(args, rank, world, local_rank):
            "ms_per_step": ms, "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16",
            "data": "synthetic", "kernel_summary": ksum,
            "config": {"workload": "C4 GPT-2-small-shaped decoder, 12 x (qkv, proj, fc, fc2) under K-FAC, "
-                                  "8 x 1024 tokens, bf16 autocast, use_true_bf16, damping 1e-3, batched_qr",
+                                  "8 x 1024 tokens, bf16 autocast, use_true_bf16, damping 1e-3, batched_qr" +
+                                  (", activations in 8 bits" if args.act8 else ""),
                       "layers_under_kfac": len(opt.hooks.linear_layers), "final_loss": float(loss.item()),
+                      "peak_mem_gb": torch.cuda.max_memory_allocated(dev) / 1e9,
                       "timing": "eager, CUDA events around the step loop (host work included)"},
            "clocks": clk.summary()}
     opt.cleanup()
@@ -1393,6 +1401,8 @@ def main():
                          "c4: the GPT-2-small-shaped decoder training step; c5: the Llama-1B-shaped one, data parallel "
                          "over the ranks; "
                          "laplace: K-FAC Laplace draws")
+    ap.add_argument("--act8", action="store_true",
+                    help="c4: hold the activations in 8 bits (Linear8, LayerNorm8, capture_8bit)")
     ap.add_argument("--c5-batch", type=int, default=2,
                     help="c5: sequences of 2048 tokens per GPU (config 5: 16 on 8 GPUs, i.e. 2 per GPU)")
     ap.add_argument("--c5-rows", choices=["all", "2048"], default="all",

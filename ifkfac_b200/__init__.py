@@ -19,4 +19,7 @@ def __getattr__(name):
     if name in ("RawActivationHooks", "IFKFACRankError"):
         from . import activation_hooks as ah
         return getattr(ah, name)
+    if name in ("Linear8", "LayerNorm8", "Q8Rows"):
+        from . import checkpoint8
+        return getattr(checkpoint8, name)
     raise AttributeError(name)

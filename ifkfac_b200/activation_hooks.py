@@ -25,7 +25,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .engine import Factor, Rows, as_rows, fold_segments
+from .checkpoint8 import Linear8
+from .engine import Factor, PackedRows, Rows, as_rows, fold_segments
 
 logger = logging.getLogger(__name__)
 
@@ -96,7 +97,7 @@ def prepare_g(delta: torch.Tensor, module: nn.Module, max_seq_rows: int, transfo
 
 
 def _rows_count(c) -> int:
-    return c.rows if isinstance(c, Rows) else int(c.shape[0])
+    return c.rows if isinstance(c, (Rows, PackedRows)) else int(c.shape[0])
 
 
 class RawActivationHooks:
@@ -105,16 +106,26 @@ class RawActivationHooks:
     Parameters are those of the reference (ifkfac/activation_hooks.py:128-216);
     ``precision`` selects the fold arithmetic (``_lib.PREC_AUTO``: tensor cores
     for bf16 chunks, fp32 CUDA cores for fp32 chunks).
+
+    ``capture_8bit`` (batched and deferred modes) keeps the pending rows in 8 bits,
+    one byte an element and one a group of 32 (``ifkfac_b200.checkpoint8``), until
+    their fold; next to a ``Linear8`` layer, X is that layer's own 8-bit input, kept
+    once for the weight gradient and the factor.  The factors are then those of the
+    rounded rows.  Conv2d inputs, which the folds read through im2col, stay images.
     """
 
     _SEQ_SUBSAMPLE: int = 2048
+    # values unpacked from 8 bits at a time, for one fold call
+    _UNPACK_BYTES: int = 1 << 30
 
     def __init__(self, model: nn.Module, damping: float = 1e-2, max_out_dim: int = 0,
                  augment_bias: bool = False, max_conv_rows: int = 512,
                  max_seq_rows: Optional[int] = None, batched: bool = False, deferred: bool = False,
-                 deferred_window: int = 5, precision: int = _lib.PREC_AUTO):
+                 deferred_window: int = 5, precision: int = _lib.PREC_AUTO, capture_8bit: bool = False):
         if batched and deferred:
             raise ValueError("batched and deferred modes are mutually exclusive")
+        if capture_8bit and not (batched or deferred):
+            raise ValueError("capture_8bit keeps pending rows: it needs batched or deferred mode")
         self.model = model
         self.damping = damping
         self.augment_bias = augment_bias
@@ -124,6 +135,7 @@ class RawActivationHooks:
         self.deferred = deferred
         self.deferred_window = deferred_window
         self.precision = precision
+        self.capture_8bit = capture_8bit
         self.chunk_transform_X = None
         self.chunk_transform_G = None
         self._handles: List = []
@@ -179,6 +191,8 @@ class RawActivationHooks:
         for module in self._linear_layers:
             self._handles.append(module.register_forward_hook(self._forward_hook))
             self._handles.append(module.register_full_backward_hook(self._backward_hook))
+            if self.capture_8bit and isinstance(module, Linear8):
+                module._share_rows = True
         self._enabled = True
 
     def pause(self) -> None:
@@ -226,9 +240,28 @@ class RawActivationHooks:
         the deferred drain of :347-364).  With an explicit precision the chunks may
         mix fp32 and bf16 (each segment carries its type); with PREC_AUTO the
         precision follows the chunk type, so the dtypes fold in separate calls."""
+        batch, size = [], 0
+        for e in entries:
+            # rows kept in 8 bits are unpacked for the call that folds them: a share of the entries at a time
+            add = sum(4 * c.rows * c.cols for c in e[2] if isinstance(c, PackedRows))
+            if batch and size + add > self._UNPACK_BYTES:
+                self._fold_batch(batch)
+                batch, size = [], 0
+            batch.append(e)
+            size += add
+        if batch:
+            self._fold_batch(batch)
+
+    def _rows_of(self, c) -> Rows:
+        if isinstance(c, PackedRows):
+            # exact in either dtype: bf16 unless the precision follows the captured one
+            return c.unpack(None if self.precision == _lib.PREC_AUTO else torch.bfloat16)
+        return as_rows(c)
+
+    def _fold_batch(self, entries) -> None:
         groups: Dict[Tuple, List] = {}
         for table, module, chunks in entries:
-            rs = [as_rows(c) for c in chunks]
+            rs = [self._rows_of(c) for c in chunks]
             rs = [r for r in rs if r.rows > 0]
             if not rs:
                 continue
@@ -246,10 +279,13 @@ class RawActivationHooks:
 
     # ---- hooks ----
     def _forward_hook(self, module, inp, out):
+        shared = module.take_rows() if isinstance(module, Linear8) else None
         if not self._enabled:
             return
         x = prepare_x(inp[0].detach(), module, self.max_conv_rows, self.max_seq_rows,
                       self.augment_bias, self.chunk_transform_X)
+        if self.capture_8bit and shared is not None and self.chunk_transform_X is None:
+            x = PackedRows.share(shared, x)
         self._accumulate(module, x, self._fx, self._n_rows_X, self._pending_X, self._raw_X)
 
     def _backward_hook(self, module, grad_input, grad_output):
@@ -259,6 +295,8 @@ class RawActivationHooks:
         self._accumulate(module, d, self._fg, self._n_rows_G, self._pending_G, self._raw_G)
 
     def _accumulate(self, module, chunk, table, nrows, pending, raw):
+        if self.capture_8bit and not isinstance(chunk, PackedRows) and not (isinstance(chunk, Rows) and chunk.geo):
+            chunk = PackedRows.pack(chunk)
         n = _rows_count(chunk)
         if self.deferred:
             raw[module].append(chunk)
@@ -379,5 +417,9 @@ class RawActivationHooks:
         for h in self._handles:
             h.remove()
         self._handles.clear()
+        for module in self._linear_layers:
+            if isinstance(module, Linear8):
+                module._share_rows = False
+                module.take_rows()
         self._enabled = False
         self.clear()

@@ -18,6 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import check
+from .checkpoint8 import Q8Rows, dequantize_rows, quantize_rows
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -204,6 +205,45 @@ class Rows:
         if self.ones:
             y = torch.cat([y, torch.ones(y.shape[0], 1, device=y.device, dtype=y.dtype)], dim=1)
         return y
+
+
+class PackedRows:
+    """Rows kept in 8 bits (:class:`ifkfac_b200.checkpoint8.Q8Rows`) until their fold, of
+    the captured dtype ``dtype``, with a column of ones appended when ``ones``."""
+
+    def __init__(self, q: Q8Rows, dtype: torch.dtype, ones: bool = False):
+        self.q, self.dtype, self.ones = q, dtype, bool(ones)
+
+    @property
+    def rows(self) -> int:
+        return self.q.rows
+
+    @property
+    def cols(self) -> int:
+        return self.q.cols + (1 if self.ones else 0)
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def unpack(self, dtype: Optional[torch.dtype] = None) -> Rows:
+        """The rows' values (exact in bf16 and fp32) as rows of a tensor."""
+        return Rows(dequantize_rows(self.q, dtype or self.dtype), ones=self.ones)
+
+    @classmethod
+    def pack(cls, c) -> "PackedRows":
+        """A tensor or :class:`Rows` in 8 bits; its index is applied, so only the rows
+        that will be folded are kept."""
+        r = as_rows(c)
+        return cls(quantize_rows(r.x, index=r.index), r.dtype, ones=r.ones)
+
+    @classmethod
+    def share(cls, q: Q8Rows, r: Rows) -> "PackedRows":
+        """``r`` when its tensor's rows are held as ``q`` already: those rows themselves,
+        or a copy of the ones that ``r.index`` picks."""
+        if r.index is not None:
+            q = Q8Rows(q.codes[r.index], q.scales[r.index], q.cols)
+        return cls(q, r.dtype, ones=r.ones)
 
 
 def as_rows(c) -> Rows:

@@ -56,7 +56,7 @@ class IFKFAC(torch.optim.Optimizer):
                  augment_bias: bool = False, max_conv_rows: int = 512,
                  max_seq_rows: Optional[int] = None, batched_qr: bool = False,
                  deferred_qr: bool = False, use_true_bf16: bool = False,
-                 precision: int = _lib.PREC_AUTO):
+                 precision: int = _lib.PREC_AUTO, capture_8bit: bool = False):
         self.use_true_bf16 = use_true_bf16
         params = []
         for module in model.modules():
@@ -77,7 +77,8 @@ class IFKFAC(torch.optim.Optimizer):
         self.hooks = RawActivationHooks(model, damping=damping, max_out_dim=max_out_dim,
                                         augment_bias=augment_bias, max_conv_rows=max_conv_rows,
                                         max_seq_rows=max_seq_rows, batched=batched_qr,
-                                        deferred=deferred_qr, precision=precision)
+                                        deferred=deferred_qr, precision=precision,
+                                        capture_8bit=capture_8bit)
         self.hooks.enable()
         self._factors: Dict[nn.Module, Tuple[torch.Tensor, torch.Tensor]] = {}
         self._classic_fallback: Dict = {}

@@ -191,3 +191,16 @@ def test_convert_keeps_parameters_and_structure():
     assert type(c8.convert(nn.Linear(4, 4))) is c8.Linear8
     with pytest.raises(ValueError):
         c8.LayerNorm8((4, 8))
+
+
+def test_capture_8bit_needs_a_mode_that_keeps_rows():
+    from ifkfac_b200.activation_hooks import RawActivationHooks
+    model = nn.Sequential(nn.Linear(4, 4))
+    with pytest.raises(ValueError, match="batched or deferred"):
+        RawActivationHooks(model, capture_8bit=True)
+    RawActivationHooks(model, capture_8bit=True, deferred=True)
+    hooks = RawActivationHooks(model, capture_8bit=True, batched=True)
+    hooks.enable()
+    with pytest.raises(ValueError, match="CUDA"):
+        model(torch.randn(3, 4))
+    hooks.remove()
