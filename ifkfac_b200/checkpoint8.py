@@ -29,7 +29,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from ._lib import check
+from ._lib import IFKError
 
 __all__ = ["Q8Rows", "quantize_rows", "dequantize_rows", "weight_grad", "LayerNormSaved", "layer_norm_forward",
            "layer_norm_backward", "Linear8", "LayerNorm8", "convert"]
@@ -60,38 +60,31 @@ def _need_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
-class _On:
-    """The device of a call made current, where it is not already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, dev: torch.device):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name: str, dev: torch.device, *args) -> None:
+    """A library call on the current stream of ``dev``, which is made current for it."""
+    fn = getattr(_lib.lib(), name)
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        raise IFKError(rc, name)
 
 
-def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
-    """Row-major with unit column stride (leading dimension = stride(0))."""
+def _rows2d(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(t, rows, columns, leading dimension) of row-major rows with unit column stride; a
+    tensor of any other layout is copied.  A single row's stride is not used."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D rows, got shape {tuple(t.shape)}")
-    if t.shape[1] == 0:
+    rows, cols = t.shape
+    if cols == 0:
         raise ValueError(f"{what} has no columns")
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        t = t.contiguous()
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Leading dimension; a single row's stride is not used and may be anything."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    ld, unit = t.stride()
+    if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
+        t, ld = t.contiguous(), cols
+    return t, rows, cols, max(ld, cols)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -101,41 +94,74 @@ def _ptr(t: Optional[torch.Tensor]):
 class Q8Rows:
     """Rows in 8 bits: ``codes`` (rows x pitch int8, pitch = ``cols`` rounded up to a
     multiple of 32), ``scales`` (rows x pitch / 32 uint8).  Slices along the rows are
-    views of the same storage."""
+    views of the same storage.
 
-    __slots__ = ("codes", "scales", "cols")
+    Rows made here keep codes and scales in one buffer, ``data`` (the codes of all
+    rows, then the scales)."""
+
+    __slots__ = ("rows", "cols", "data", "_codes", "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
         cols = int(cols)
         pitch = -(-cols // _G) * _G
-        if cols < 1 or codes.dim() != 2 or scales.dim() != 2 or codes.shape != (scales.shape[0], pitch) \
-                or scales.shape[1] != pitch // _G:
+        rows = codes.shape[0] if codes.dim() == 2 else -1
+        if cols < 1 or codes.shape != (rows, pitch) or scales.shape != (rows, pitch // _G):
             raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not rows of {cols} "
                              f"columns (rows x {pitch} and rows x {pitch // _G})")
         if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
             raise TypeError(f"8-bit rows are int8 codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
-        if codes.shape[0] > 1 and (codes.stride(0) < pitch or scales.stride(0) < pitch // _G) \
-                or codes.stride(1) != 1 or (scales.stride(1) != 1 and scales.shape[1] > 1):
+        (ldc, uc), (lds, us) = codes.stride(), scales.stride()
+        if rows > 1 and (ldc < pitch or lds < pitch // _G) or uc != 1 or (us != 1 and pitch > _G):
             raise ValueError("codes and scales must be row-major")
-        self.codes, self.scales, self.cols = codes, scales, cols
+        self.rows, self.cols, self.data, self._codes, self._scales = rows, cols, None, codes, scales
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Q8Rows":
-        pitch = -(-int(cols) // _G) * _G
-        return cls(torch.empty(rows, pitch, dtype=torch.int8, device=device),
-                   torch.empty(rows, pitch // _G, dtype=torch.uint8, device=device), cols)
+        pitch = -(-cols // _G) * _G
+        return cls.of(torch.empty(rows * (pitch + pitch // _G), dtype=torch.uint8, device=device), rows, cols)
+
+    @classmethod
+    def of(cls, data: torch.Tensor, rows: int, cols: int) -> "Q8Rows":
+        """The rows in a buffer laid out as ``data``."""
+        q = cls.__new__(cls)
+        q.rows, q.cols, q.data, q._codes, q._scales = rows, cols, data, None, None
+        return q
 
     @property
-    def rows(self) -> int:
-        return int(self.codes.shape[0])
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            pitch = -(-self.cols // _G) * _G
+            self._codes = self.data[: self.rows * pitch].view(torch.int8).view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            pitch = -(-self.cols // _G) * _G
+            self._scales = self.data[self.rows * pitch:].view(self.rows, pitch // _G)
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self.data is None else self.data).device
 
     @property
     def nbytes(self) -> int:
-        return self.rows * (self.codes.shape[1] + self.scales.shape[1])
+        pitch = -(-self.cols // _G) * _G
+        return self.rows * (pitch + pitch // _G)
+
+    def tensors(self) -> Tuple[torch.Tensor, ...]:
+        """The tensors that hold the rows."""
+        return (self._codes, self._scales) if self.data is None else (self.data,)
+
+    def args(self) -> Tuple[int, int, int, int]:
+        """(codes, ld, scales, ld) of a library call."""
+        pitch = -(-self.cols // _G) * _G
+        if self.data is not None:
+            p = self.data.data_ptr()
+            return p, pitch, p + self.rows * pitch, pitch // _G
+        c, s = self._codes, self._scales
+        return c.data_ptr(), max(c.stride(0), pitch), s.data_ptr(), max(s.stride(0), pitch // _G)
 
     def __getitem__(self, rows: slice) -> "Q8Rows":
         if not isinstance(rows, slice) or rows.step not in (None, 1):
@@ -146,17 +172,10 @@ class Q8Rows:
         return f"Q8Rows({self.rows} x {self.cols}, {self.device})"
 
 
-def _index(index: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]:
-    if index is None:
-        return None
+def _index(index: torch.Tensor, dev: torch.device) -> torch.Tensor:
     if index.dim() != 1 or index.dtype not in (torch.int64, torch.int32):
         raise ValueError("a row index is a 1-D integer tensor")
     return index.to(device=dev, dtype=torch.int64).contiguous()
-
-
-def _q8(q: Q8Rows):
-    """(codes, ld, scales, ld) of a call's arguments."""
-    return q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(), _ld(q.scales)
 
 
 def quantize_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None,
@@ -167,28 +186,29 @@ def quantize_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None,
     group that holds a NaN or an infinity reads back as NaN.  An index outside x
     gives a zero row and IFK_ERR_ARG in ``status`` (a device int32, optional)."""
     dev = _need_cuda(x, status)
-    x = _rows2d(x, "x")
+    x, src, cols, ld = _rows2d(x, "x")
     dt = _code(x.dtype)
-    index = _index(index, dev)
-    rows = x.shape[0] if index is None else index.numel()
-    with _On(dev) as stream:
-        q = Q8Rows.empty(rows, x.shape[1], dev)
-        check(_lib.lib().ifk_q8_quantize(x.data_ptr(), _ld(x), dt, _ptr(index), x.shape[0], rows, x.shape[1], *_q8(q),
-                                         _ptr(status), stream), "ifk_q8_quantize")
+    rows = src
+    if index is not None:
+        index = _index(index, dev)
+        rows = index.numel()
+    q = Q8Rows.empty(rows, cols, dev)
+    _call("ifk_q8_quantize", dev, x.data_ptr(), ld, dt, _ptr(index), src, rows, cols, *q.args(), _ptr(status))
     return q
 
 
 def dequantize_rows(q: Q8Rows, dtype: torch.dtype = torch.bfloat16, index: Optional[torch.Tensor] = None,
                     status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of 8-bit rows (or of the rows ``index`` of them), exact in either dtype."""
-    dev = _need_cuda(q.codes, q.scales, status)
+    dev = _need_cuda(*q.tensors(), status)
     dt = _code(dtype)
-    index = _index(index, dev)
-    rows = q.rows if index is None else index.numel()
-    with _On(dev) as stream:
-        out = torch.empty(rows, q.cols, dtype=dtype, device=dev)
-        check(_lib.lib().ifk_q8_dequantize(*_q8(q), _ptr(index), q.rows, rows, q.cols, out.data_ptr(), q.cols, dt,
-                                           _ptr(status), stream), "ifk_q8_dequantize")
+    rows = q.rows
+    if index is not None:
+        index = _index(index, dev)
+        rows = index.numel()
+    out = torch.empty(rows, q.cols, dtype=dtype, device=dev)
+    _call("ifk_q8_dequantize", dev, *q.args(), _ptr(index), q.rows, rows, q.cols, out.data_ptr(), q.cols, dt,
+          _ptr(status))
     return out
 
 
@@ -199,51 +219,67 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
     from the 8-bit rows of X, and with ``bias`` (or ``out_bias``) db = the column sums
     of delta, else None.  ``out`` / ``out_bias`` receive them; with ``accumulate`` they
     are added to (gradient accumulation), and both that are wanted must be given."""
-    dev = _need_cuda(delta, q.codes, q.scales, out, out_bias, status)
-    delta = _rows2d(delta, "delta")
+    dev = _need_cuda(delta, *q.tensors(), out, out_bias, status)
+    delta, rows, n_out, ld = _rows2d(delta, "delta")
     dt = _code(delta.dtype)
-    rows, n_out = delta.shape
+    n_in = q.cols
     if rows != q.rows:
         raise ValueError(f"delta has {rows} rows, the layer's input {q.rows}")
     if accumulate and (out is None or (bias and out_bias is None)):
         raise ValueError("accumulate needs the tensors to add to")
-    with _On(dev) as stream:
-        if out is None:
-            out = torch.empty(n_out, q.cols, dtype=torch.float32, device=dev)
-        elif out.dtype != torch.float32 or out.shape != (n_out, q.cols) or out.stride(1) != 1 \
-                or (n_out > 1 and out.stride(0) < q.cols):
-            raise ValueError(f"out must be a row-major {n_out} x {q.cols} float32 tensor")
-        if out_bias is None and bias:
+    ld_out = n_in
+    if out is None:
+        out = torch.empty(n_out, n_in, dtype=torch.float32, device=dev)
+    else:
+        if out.dtype != torch.float32 or out.shape != (n_out, n_in) or (out.stride(1) != 1 and n_in > 1) \
+                or (n_out > 1 and out.stride(0) < n_in):
+            raise ValueError(f"out must be a row-major {n_out} x {n_in} float32 tensor")
+        ld_out = max(out.stride(0), n_in)
+    if out_bias is None:
+        if bias:
             out_bias = torch.empty(n_out, dtype=torch.float32, device=dev)
-        elif out_bias is not None and (out_bias.dtype != torch.float32 or out_bias.shape != (n_out,)
-                                       or not out_bias.is_contiguous()):
-            raise ValueError(f"out_bias must be a contiguous float32 tensor of {n_out}")
-        L = _lib.lib()
-        ws = torch.empty(L.ifk_q8_wgrad_workspace(rows, n_out, q.cols, dt), dtype=torch.uint8, device=dev)
-        check(L.ifk_q8_wgrad(delta.data_ptr(), _ld(delta), dt, *_q8(q), rows, n_out, q.cols, out.data_ptr(), _ld(out),
-                             _ptr(out_bias), 1 if accumulate else 0, _ptr(status), ws.data_ptr(), ws.numel(), stream),
-              "ifk_q8_wgrad")
+    elif out_bias.dtype != torch.float32 or out_bias.shape != (n_out,) or not out_bias.is_contiguous():
+        raise ValueError(f"out_bias must be a contiguous float32 tensor of {n_out}")
+    nbytes = _lib.lib().ifk_q8_wgrad_workspace(rows, n_out, n_in, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("ifk_q8_wgrad", dev, delta.data_ptr(), ld, dt, *q.args(), rows, n_out, n_in, out.data_ptr(), ld_out,
+          _ptr(out_bias), 1 if accumulate else 0, _ptr(status), ws.data_ptr(), nbytes)
     return out, out_bias
 
 
 class LayerNormSaved:
-    """What layer norm's backward pass needs of its forward pass: the statistics and
-    the input rows, as they were (``x``) or in 8 bits (``q8``)."""
+    """What layer norm's backward pass needs of its forward pass: the statistics (``stats``,
+    2 x rows fp32: means, then reciprocal deviations) and the input rows, as they were
+    (``x``) or in 8 bits (``q8``)."""
 
-    __slots__ = ("x", "q8", "mean", "rstd", "x_dtype", "cols")
+    __slots__ = ("x", "q8", "stats", "x_dtype", "rows", "cols")
 
-    def __init__(self, x, q8, mean, rstd, x_dtype, cols):
-        self.x, self.q8, self.mean, self.rstd, self.x_dtype, self.cols = x, q8, mean, rstd, x_dtype, cols
+    def __init__(self, x: Optional[torch.Tensor], q8: Optional[Q8Rows], stats: torch.Tensor, x_dtype: torch.dtype,
+                 rows: int, cols: int):
+        self.x, self.q8, self.stats, self.x_dtype, self.rows, self.cols = x, q8, stats, x_dtype, rows, cols
+
+    @property
+    def mean(self) -> torch.Tensor:
+        return self.stats[0]
+
+    @property
+    def rstd(self) -> torch.Tensor:
+        return self.stats[1]
 
 
-def _affine(n: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.shape != (n,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must hold {n} contiguous values, got shape {tuple(t.shape)}")
+def _affine(n: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
+    t = weight if weight is not None else bias
+    if t is None:
+        return _lib.F32
+    for p, name in ((weight, "weight"), (bias, "bias")):
+        if p is not None and (p.shape != (n,) or not p.is_contiguous()):
+            raise ValueError(f"{name} must hold {n} contiguous values, got shape {tuple(p.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight and bias share a dtype, got {weight.dtype} and {bias.dtype}")
-    t = weight if weight is not None else bias
-    return _lib.F32 if t is None else _code(t.dtype)
+    return _code(t.dtype)
+
+
+_NO_ROWS = (None, 0, None, 0)
 
 
 def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -254,24 +290,26 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     :func:`layer_norm_backward` needs; with ``checkpoint`` the input is held there
     in 8 bits, written in the same pass, instead of as itself."""
     dev = _need_cuda(x, weight, bias)
-    x = _rows2d(x, "x")
+    x, rows, n, ld = _rows2d(x, "x")
     dt = _code(x.dtype)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype is None:
+        out_dtype = x.dtype
     ydt = _code(out_dtype)
-    rows, n = x.shape
     wdt = _affine(n, weight, bias)
+    y = torch.empty(rows, n, dtype=out_dtype, device=dev)
     saved = mean = rstd = None
-    q = (None, 0, None, 0)
-    with _On(dev) as stream:
-        y = torch.empty(rows, n, dtype=out_dtype, device=dev)
-        if save:
-            mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=dev)
-            rows8 = Q8Rows.empty(rows, n, dev) if checkpoint else None
-            saved = LayerNormSaved(None if checkpoint else x, rows8, mean, rstd, x.dtype, n)
-            if checkpoint:
-                q = _q8(rows8)
-        check(_lib.lib().ifk_layernorm(x.data_ptr(), _ld(x), dt, _ptr(weight), _ptr(bias), wdt, rows, n, float(eps),
-                                       y.data_ptr(), n, ydt, _ptr(mean), _ptr(rstd), *q, stream), "ifk_layernorm")
+    q = _NO_ROWS
+    if save:
+        stats = torch.empty(2, rows, dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+        q8 = None
+        if checkpoint:
+            q8 = Q8Rows.empty(rows, n, dev)
+            q = q8.args()
+        saved = LayerNormSaved(None if checkpoint else x, q8, stats, x.dtype, rows, n)
+    _call("ifk_layernorm", dev, x.data_ptr(), ld, dt, _ptr(weight), _ptr(bias), wdt, rows, n, float(eps),
+          y.data_ptr(), n, ydt, mean, rstd, *q)
     return y, saved
 
 
@@ -280,27 +318,27 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw, db) of :func:`layer_norm_forward`: dx in the input's dtype, dw and db
     fp32 (None without ``weight_grads``)."""
-    dev = _need_cuda(dy, saved.mean, weight)
-    dy = _rows2d(dy, "dy")
+    dev = _need_cuda(dy, saved.stats, weight)
+    dy, rows, n, ld = _rows2d(dy, "dy")
     dt, xdt = _code(dy.dtype), _code(saved.x_dtype)
-    rows, n = dy.shape
-    if (rows, n) != (saved.mean.numel(), saved.cols):
-        raise ValueError(f"dy is {rows} x {n}, the input was {saved.mean.numel()} x {saved.cols}")
+    if rows != saved.rows or n != saved.cols:
+        raise ValueError(f"dy is {rows} x {n}, the input was {saved.rows} x {saved.cols}")
     wdt = _affine(n, weight, None)
-    x, q = saved.x, (None, 0, None, 0)
-    if x is None:
-        q = _q8(saved.q8)
-    with _On(dev) as stream:
-        L = _lib.lib()
-        dx = torch.empty(rows, n, dtype=saved.x_dtype, device=dev)
-        dw = db = ws = None
-        if weight_grads:
-            dw, db = torch.empty(2, n, dtype=torch.float32, device=dev)
-            ws = torch.empty(L.ifk_layernorm_backward_workspace(rows, n), dtype=torch.uint8, device=dev)
-        check(L.ifk_layernorm_backward(
-            dy.data_ptr(), _ld(dy), dt, _ptr(x), 0 if x is None else _ld(x), xdt, *q, saved.mean.data_ptr(),
-            saved.rstd.data_ptr(), _ptr(weight), wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(ws),
-            0 if ws is None else ws.numel(), stream), "ifk_layernorm_backward")
+    if saved.x is None:
+        x, ldx, q = None, 0, saved.q8.args()
+    else:
+        x, ldx, q = saved.x.data_ptr(), max(saved.x.stride(0), n), _NO_ROWS
+    dx = torch.empty(rows, n, dtype=saved.x_dtype, device=dev)
+    dw = db = ws = None
+    nbytes = 0
+    if weight_grads:
+        dw = torch.empty(n, dtype=torch.float32, device=dev)
+        db = torch.empty(n, dtype=torch.float32, device=dev)
+        nbytes = _lib.lib().ifk_layernorm_backward_workspace(rows, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    mean = saved.stats.data_ptr()
+    _call("ifk_layernorm_backward", dev, dy.data_ptr(), ld, dt, x, ldx, xdt, *q, mean, mean + 4 * rows, _ptr(weight),
+          wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(ws), nbytes)
     return dx, dw, db
 
 
@@ -316,9 +354,8 @@ class _LinearQ8(torch.autograd.Function):
         with torch.autocast("cuda", enabled=False):
             w = weight.to(dtype)
             y = F.linear(x.to(dtype), w, None if bias is None else bias.to(dtype))
-        saved = [] if q is None else [q.codes, q.scales]
-        ctx.save_for_backward(w, *saved)
-        ctx.cols, ctx.x_shape, ctx.x_dtype = x.shape[-1], x.shape, x.dtype
+        ctx.save_for_backward(w, *(() if q is None else (q.data,)))
+        ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         ctx.w_dtype, ctx.b_dtype = weight.dtype, None if bias is None else bias.dtype
         return y
 
@@ -332,7 +369,8 @@ class _LinearQ8(torch.autograd.Function):
             if ctx.needs_input_grad[0]:
                 dx = (d2 @ w).reshape(ctx.x_shape).to(ctx.x_dtype)
             if ctx.needs_input_grad[1]:
-                dw, db = weight_grad(d2, Q8Rows(*saved, ctx.cols), bias=ctx.needs_input_grad[2])
+                q = Q8Rows.of(saved[0], d2.shape[0], ctx.x_shape[-1])
+                dw, db = weight_grad(d2, q, bias=ctx.needs_input_grad[2])
                 dw = dw.to(ctx.w_dtype)
                 db = None if db is None else db.to(ctx.b_dtype)
             elif ctx.needs_input_grad[2]:
@@ -381,7 +419,7 @@ class _LayerNormQ8(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, dtype, save):
         y, s = layer_norm_forward(x.reshape(-1, x.shape[-1]), weight, bias, eps, dtype, save=save, checkpoint=True)
         if s is not None:
-            ctx.save_for_backward(s.mean, s.rstd, s.q8.codes, s.q8.scales, *(() if weight is None else (weight,)))
+            ctx.save_for_backward(s.stats, s.q8.data, *(() if weight is None else (weight,)))
         ctx.x_dtype, ctx.x_shape = x.dtype, x.shape
         ctx.b_dtype = None if bias is None else bias.dtype
         return y.reshape(x.shape)
@@ -389,9 +427,9 @@ class _LayerNormQ8(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        mean, rstd, codes, scales, *w = ctx.saved_tensors
-        n = ctx.x_shape[-1]
-        saved = LayerNormSaved(None, Q8Rows(codes, scales, n), mean, rstd, ctx.x_dtype, n)
+        stats, data, *w = ctx.saved_tensors
+        rows, n = stats.shape[1], ctx.x_shape[-1]
+        saved = LayerNormSaved(None, Q8Rows.of(data, rows, n), stats, ctx.x_dtype, rows, n)
         weight = w[0] if w else None
         dx, dw, db = layer_norm_backward(dy.reshape(-1, n), saved, weight,
                                          weight_grads=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
