@@ -15,6 +15,7 @@ bool aligned(const void* p) { return ((uintptr_t)p % ALIGN) == 0; }
 bool dtype_ok(int d) { return d == IFK_F32 || d == IFK_BF16; }
 cudaStream_t S(ifk_stream_t s) { return (cudaStream_t)s; }
 
+// Largest width, and largest side of a weight gradient: columns and tiles are 32-bit in the kernels.
 constexpr int64_t MAX_SIDE = 1 << 28;
 
 // Layout of 8-bit rows of n columns.
@@ -33,7 +34,7 @@ int64_t ifk_q8_pitch(int64_t n) { return n <= 0 ? 0 : q8::pitch(n); }
 int ifk_q8_quantize(const void* x, int64_t ld_x, int dtype, const int64_t* row_index, int64_t src_rows, int64_t rows,
                     int64_t n, int8_t* codes, int64_t ld_codes, uint8_t* scales, int64_t ld_scales, int* d_status,
                     ifk_stream_t stream) {
-  if (rows < 0 || n <= 0) return IFK_ERR_SHAPE;
+  if (rows < 0 || n <= 0 || n > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(dtype)) return IFK_ERR_DTYPE;
   if (rows == 0) return IFK_OK;
   if (!x) return IFK_ERR_ARG;
@@ -47,7 +48,7 @@ int ifk_q8_quantize(const void* x, int64_t ld_x, int dtype, const int64_t* row_i
 int ifk_q8_dequantize(const int8_t* codes, int64_t ld_codes, const uint8_t* scales, int64_t ld_scales,
                       const int64_t* row_index, int64_t src_rows, int64_t rows, int64_t n, void* out, int64_t ld_out,
                       int out_dtype, int* d_status, ifk_stream_t stream) {
-  if (rows < 0 || n <= 0) return IFK_ERR_SHAPE;
+  if (rows < 0 || n <= 0 || n > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(out_dtype)) return IFK_ERR_DTYPE;
   if (rows == 0) return IFK_OK;
   if (!out) return IFK_ERR_ARG;
@@ -70,7 +71,7 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
                  ifk_stream_t stream) {
   if (!dW) return IFK_ERR_ARG;
   if (rows < 0 || n_out <= 0 || n_in <= 0 || ld_dW < n_in) return IFK_ERR_SHAPE;
-  if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return IFK_ERR_SHAPE;  // 32-bit tile coordinates
+  if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(delta_dtype)) return IFK_ERR_DTYPE;
   cudaStream_t s = S(stream);
   if (rows == 0) {
@@ -94,7 +95,7 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
 int ifk_layernorm(const void* x, int64_t ld_x, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,
                   int64_t n, double eps, void* y, int64_t ld_y, int y_dtype, float* mean, float* rstd, int8_t* codes,
                   int64_t ld_codes, uint8_t* scales, int64_t ld_scales, ifk_stream_t stream) {
-  if (rows < 0 || n <= 0) return IFK_ERR_SHAPE;
+  if (rows < 0 || n <= 0 || n > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype) || ((w || b) && !dtype_ok(w_dtype))) return IFK_ERR_DTYPE;
   if (!(eps >= 0) || std::isinf(eps)) return IFK_ERR_ARG;
   if (rows == 0) return IFK_OK;
@@ -109,7 +110,7 @@ int ifk_layernorm(const void* x, int64_t ld_x, int x_dtype, const void* w, const
 }
 
 size_t ifk_layernorm_backward_workspace(int64_t rows, int64_t n) {
-  if (rows < 0 || n <= 0) return 0;
+  if (rows < 0 || n <= 0 || n > MAX_SIDE) return 0;
   return align_up(layernorm_backward_bytes(rows, n));
 }
 
@@ -118,7 +119,7 @@ int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const voi
                            const float* mean, const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n,
                            void* dx, int64_t ld_dx, float* dw, float* db, void* workspace, size_t workspace_bytes,
                            ifk_stream_t stream) {
-  if (rows < 0 || n <= 0) return IFK_ERR_SHAPE;
+  if (rows < 0 || n <= 0 || n > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (w && !dtype_ok(w_dtype))) return IFK_ERR_DTYPE;
   cudaStream_t s = S(stream);
   if (rows == 0) {

@@ -49,9 +49,9 @@ __device__ __forceinline__ float team_sum(float v, int W, float* buf) {
 // 8-bit rows of x, written as ifk_q8_quantize writes them.
 template <int V>
 __device__ __forceinline__ void write_codes(const FwdArgs& a, int64_t row, int c, const float (&v)[V]) {
-  const uint32_t s = q8::scale_byte(q8::group_max_bits<V>(v));
+  const uint32_t m = q8::group_max_bits<V>(v), s = q8::scale_byte(m);
   if (c >= a.pitch) return;
-  q8::store_codes<V>(a.codes + row * a.ldc + c, v, s);
+  q8::store_codes<V>(a.codes + row * a.ldc + c, v, m, s);
   if ((c & (q8::GROUP - 1)) == 0) a.scales[row * a.lds + c / q8::GROUP] = (uint8_t)s;
 }
 

@@ -8,7 +8,6 @@ namespace ifk {
 namespace q8 {
 
 constexpr int GROUP = IFK_Q8_GROUP;
-constexpr int VEC = 8;  // columns a thread holds: 4 neighbouring lanes make a group
 
 __host__ __device__ inline int64_t pitch(int64_t n) { return cdiv(n, GROUP) * GROUP; }
 
@@ -25,34 +24,16 @@ __device__ __forceinline__ float inv_scale(uint32_t s) { return __uint_as_float(
 // 2^e, or +inf for byte 255, whose codes are 0: 0 * inf reads as NaN.
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
 
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// Whether a code of the group can round to 128 and has to be clipped: the largest |x| 2^-e is 127.5 or more.
+__device__ __forceinline__ bool may_clip(uint32_t amax_bits) { return (amax_bits & 0x007fffffu) >= 0x007f0000u; }
 
-// The largest |x| of a group whose 32 columns lie in 4 neighbouring lanes (of a
-// 4-aligned quad), as bits: integer order is the order of magnitudes, with NaN on top.
-__device__ __forceinline__ uint32_t group_max(const float (&x)[VEC]) {
-  uint32_t a = abs_bits(x[0]);
-#pragma unroll
-  for (int i = 1; i < VEC; ++i) a = max(a, abs_bits(x[i]));
-  a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  return max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-}
-
-// code of x: rint(x 2^-e) clipped to +-127, as the low byte of the fp32 bits of
-// code + 1.5 * 2^23 (the addition rounds to the nearest integer, ties to even).
+// code of x as the low byte of the fp32 bits of code + 1.5 * 2^23: x 2^-e is exact, and the addition rounds
+// to the nearest integer, ties to even.
 __device__ __forceinline__ uint32_t code_bits(float x, float inv) {
-  const float v = fminf(fmaxf(x * inv, -127.f), 127.f);
-  return __float_as_uint(v + 12582912.f);
+  return __float_as_uint(fmaf(x, inv, 12582912.f));
 }
-__device__ __forceinline__ uint2 codes8(const float (&x)[VEC], uint32_t s) {
-  if (s == 255u) return make_uint2(0u, 0u);
-  const float inv = inv_scale(s);
-  uint32_t b[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) b[i] = code_bits(x[i], inv);
-  uint2 r;
-  r.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-  r.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-  return r;
+__device__ __forceinline__ uint32_t code_bits_clipped(float x, float inv) {
+  return __float_as_uint(fminf(fmaxf(x * inv, -127.f), 127.f) + 12582912.f);
 }
 
 // The value of one of four packed codes: the byte with its sign bit flipped is
@@ -60,14 +41,6 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[VEC], uint32_t s) {
 __device__ __forceinline__ float value_of(uint32_t flipped, int byte, float scale) {
   const float u = __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7540 | byte));
   return (u - 8388736.f) * scale;
-}
-__device__ __forceinline__ void values8(uint2 c, float scale, float (&v)[VEC]) {
-  const uint32_t lo = c.x ^ 0x80808080u, hi = c.y ^ 0x80808080u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = value_of(lo, i, scale);
-    v[4 + i] = value_of(hi, i, scale);
-  }
 }
 
 }  // namespace q8

@@ -130,35 +130,44 @@ __device__ __forceinline__ void load_param(const void* p, bool bf16, float none,
 
 namespace q8 {
 
-// The largest |x| of a group whose 32 columns lie V to a lane in 32 / V neighbouring lanes, as bits
-// (integer order is the order of magnitudes, NaN on top).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The largest |x| of a group whose 32 columns lie V to a lane in 32 / V neighbouring lanes, as bits; a NaN
+// comes through as one.
 template <int V>
 __device__ __forceinline__ uint32_t group_max_bits(const float (&x)[V]) {
-  uint32_t a = abs_bits(x[0]);
+  float a = fabsf(x[0]);
 #pragma unroll
-  for (int i = 1; i < V; ++i) a = max(a, abs_bits(x[i]));
+  for (int i = 1; i < V; ++i) a = max_nan(a, fabsf(x[i]));
 #pragma unroll
-  for (int o = 1; o < GROUP / V; o *= 2) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  return a;
+  for (int o = 1; o < GROUP / V; o *= 2) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return __float_as_uint(a) & 0x7fffffffu;
 }
 
-// V codes to memory (V-byte aligned).
+// V codes of a group with this largest magnitude and scale byte to memory (V-byte aligned).
 template <int V>
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&x)[V], uint32_t s) {
-  uint32_t w[(V + 3) / 4];
-  const float inv = s == 255u ? 0.f : inv_scale(s);
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&x)[V], uint32_t amax_bits, uint32_t s) {
+  uint32_t e[V], w[(V + 3) / 4];
+  if (s == 255u) {
 #pragma unroll
-  for (int j = 0; j < (V + 3) / 4; ++j) {
-    if (s == 255u) {
-      w[j] = 0u;
-    } else if (V == 1) {
-      w[j] = code_bits(x[0], inv);
-    } else {
-      const uint32_t lo = __byte_perm(code_bits(x[(4 * j) % V], inv), code_bits(x[(4 * j + 1) % V], inv), 0x0040);
-      const uint32_t hi = __byte_perm(code_bits(x[(4 * j + 2) % V], inv), code_bits(x[(4 * j + 3) % V], inv), 0x0040);
-      w[j] = __byte_perm(lo, hi, 0x5410);
-    }
+    for (int i = 0; i < V; ++i) e[i] = 0u;
+  } else if (may_clip(amax_bits)) {
+    const float inv = inv_scale(s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = code_bits_clipped(x[i], inv);
+  } else {
+    const float inv = inv_scale(s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = code_bits(x[i], inv);
   }
+#pragma unroll
+  for (int j = 0; j < (V + 3) / 4; ++j)
+    w[j] = V == 1 ? e[0]
+                  : __byte_perm(__byte_perm(e[(4 * j) % V], e[(4 * j + 1) % V], 0x0040),
+                                __byte_perm(e[(4 * j + 2) % V], e[(4 * j + 3) % V], 0x0040), 0x5410);
   if (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[(V + 3) / 4 - 1]);
   else if (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
   else *p = (int8_t)w[0];

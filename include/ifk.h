@@ -487,7 +487,7 @@ IFK_API int ifk_update_bias(float* b, const float* nat_b, int64_t count, double 
  *
  * codes is rows x ld_codes int8 with ld_codes >= ifk_q8_pitch(n) (n rounded up
  * to a multiple of 32; the columns past n are written as 0 and never used), a
- * multiple of 16, and a 16-byte aligned base; scales is rows x ld_scales uint8
+ * multiple of 16, and a 16-byte aligned base; n is at most 2^28; scales is rows x ld_scales uint8
  * with ld_scales >= ifk_q8_pitch(n) / 32.  The reference keeps such rows in
  * the dtype they were captured in (ifkfac/activation_hooks.py:560-570, 627-635).
  */
