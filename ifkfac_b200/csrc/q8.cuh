@@ -45,62 +45,4 @@ __device__ __forceinline__ float value_of(uint32_t flipped, int byte, float scal
 
 }  // namespace q8
 
-// Eight neighbouring columns of a row from column c on; columns at or past n read
-// as 0.  vec: the row is 16-byte aligned (c is a multiple of 8).
-__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t n, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= n) {
-    const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? row[c + i] : 0.f;
-  }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* row, int64_t c, int64_t n, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= n) {
-    const uint4 a = *reinterpret_cast<const uint4*>(row + c);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? __bfloat162float(row[c + i]) : 0.f;
-  }
-}
-__device__ __forceinline__ void store8(float* row, int64_t c, int64_t n, bool vec, const float (&v)[8]) {
-  if (vec && c + 8 <= n) {
-    *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) row[c + i] = v[i];
-  }
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* row, int64_t c, int64_t n, bool vec, const float (&v)[8]) {
-  if (vec && c + 8 <= n) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&p);
-    }
-    *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) row[c + i] = __float2bfloat16_rn(v[i]);
-  }
-}
-
-// Rows of a matrix of element type T: 16-byte accesses at columns that are multiples of 8.
-template <typename T>
-inline bool rows_aligned(const T* p, int64_t ld) {
-  return (((uintptr_t)p) & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
-}
-
 }  // namespace ifk

@@ -27,7 +27,10 @@
 // tile's shares in order.
 #include <cuda.h>
 
-#include "q8.cuh"
+#include <algorithm>
+#include <cstring>
+
+#include "rowvec.cuh"
 #include "ifk_internal.h"
 #include "tc.cuh"
 
@@ -85,6 +88,7 @@ struct Args {
   float* part;         // [2 Gs][TN][2 TM]
   int accumulate;
   bool vec_scales;     // rows of scales start at multiples of 4 bytes
+  bool vec_out;        // rows of dW start at multiples of 16 bytes
   bool whole;          // delta's map has 64-column blocks as a dimension (n_out a multiple of 64)
   int* status;
 };
@@ -237,6 +241,10 @@ __device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map
       "%3, %4, %5}], [%6];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(t), "r"(bar)
       : "memory");
+}
+
+__device__ __forceinline__ void red_add(float* p, float v) {
+  asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory");
 }
 
 // Operand tiles: M/N-major, 128-byte swizzle.  64 columns of 8 rows are one 1024-byte
@@ -462,7 +470,9 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
       const bool to_part = w.slot >= 0;
       float* d = to_part ? a.part + (int64_t)w.slot * (TN * 2 * TM) + m : a.dW + o0 * a.ldw + i;
       const int64_t ld = to_part ? 2 * TM : a.ldw;
-      const int cols = to_part ? TN : (i < a.n_in ? (int)mn<int64_t>(TN, a.n_out - o0) : 0);
+      const bool in = i < a.n_in;
+      // columns of the tile that dW has (none where the whole warp is past its rows' end)
+      const int cols = i - lane < a.n_in ? (int)mn<int64_t>(TN, a.n_out - o0) : 0;
       bool add = !to_part && a.accumulate;
       for (int c0 = w.k0; c0 < w.k1; c0 = chunk_end(c0, w.k1)) {
         if (!wait_bar(acc_full + 8 * buf, bph, failed)) {
@@ -470,25 +480,26 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
           break;
         }
         tc::fence_after();
-        for (int c = 0; c < TN; c += 32) {
+        for (int c = 0; c < cols; c += 32) {
           float v[32];
           tc::tmem_ld32(tmem + buf * TN + c + ((uint32_t)(wq * 32) << 16), v);
           float* p = d + c * ld;
+          if (!in) continue;
           if (c + 32 <= cols) {
             if (add) {
 #pragma unroll
-              for (int q = 0; q < 32; ++q, p += ld) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v[q]) : "memory");
+              for (int q = 0; q < 32; ++q, p += ld) red_add(p, v[q]);
             } else {
 #pragma unroll
               for (int q = 0; q < 32; ++q, p += ld) *p = v[q];
             }
           } else {
 #pragma unroll
-            for (int q = 0; q < 32; ++q, p += ld)
-              if (c + q < cols) {
-                if (add) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v[q]) : "memory");
-                else *p = v[q];
-              }
+            for (int q = 0; q < 32; ++q, p += ld) {
+              if (c + q >= cols) break;
+              if (add) red_add(p, v[q]);
+              else *p = v[q];
+            }
           }
         }
         add = true;
@@ -562,26 +573,69 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// A cut tile's shares, added in the order of the rows.  A block takes 16 output columns.
-__global__ void __launch_bounds__(2 * TM) join_kernel(const Args a) {
+// What is left when the tiles are summed.  The first `joins` blocks add a cut tile's shares, in the
+// order of the rows, 16 output columns a block: a thread has four 16-byte reads of a share in
+// flight.  The others add the parts of db, 32 columns a block.
+constexpr int JOIN_COLS = 16;
+__global__ void __launch_bounds__(256) finish_kernel(const Args a, int joins, const float* sums, int parts, float* db) {
+  if ((int)blockIdx.x >= joins) {
+    __shared__ float sh[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (int64_t)(blockIdx.x - joins) * 32 + tx;
+    float v = 0.f;
+    if (c < a.n_out)
+      for (int p = ty; p < parts; p += 8) v += sums[(int64_t)p * a.n_out + c];
+    sh[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && c < a.n_out) {
+      v = sh[0][tx];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) v += sh[q][tx];
+      db[c] = a.accumulate ? db[c] + v : v;
+    }
+    return;
+  }
   const Plan& p = a.p;
-  const int64_t t = blockIdx.x, b = t * p.Kt;
+  constexpr int PER = TN / JOIN_COLS;
+  const int64_t t = blockIdx.x / PER, b = t * p.Kt;
   const int w0 = p.owner(b), w1 = p.owner(b + p.Kt - 1);
   if (w0 == w1) return;  // one cluster had it all
-  const int tile = p.Tdp + (int)t;
-  const int64_t i = (int64_t)(tile % p.Ti) * 2 * TM + threadIdx.x;
-  const int64_t o0 = (int64_t)(tile / p.Ti) * TN + blockIdx.y * 16;
-  if (i >= a.n_in) return;
+  const int tile = p.Tdp + (int)t, o = (int)(blockIdx.x % PER) * JOIN_COLS;
+  const int64_t i = (int64_t)(tile % p.Ti) * 2 * TM + (threadIdx.x & 63) * 4;
+  const int64_t o0 = (int64_t)(tile / p.Ti) * TN + o;
   constexpr int64_t SLOT = TN * 2 * TM;
-  const float* src = a.part + (int64_t)blockIdx.y * 16 * (2 * TM) + threadIdx.x;
-#pragma unroll 4
-  for (int q = 0; q < 16; ++q) {
-    if (o0 + q >= a.n_out) break;
-    const float* s = src + q * (2 * TM);
-    float v = s[(2 * w0 + 1) * SLOT];
-    for (int c = w0 + 1; c <= w1; ++c) v += s[2 * c * SLOT];
-    float* d = a.dW + (o0 + q) * a.ldw + i;
-    *d = a.accumulate ? *d + v : v;
+  constexpr int N = JOIN_COLS / 4;
+  const float* src = a.part + (int64_t)(o + (threadIdx.x >> 6)) * (2 * TM) + (threadIdx.x & 63) * 4;
+  const int64_t oq = o0 + (threadIdx.x >> 6);
+  if (i >= a.n_in || oq >= a.n_out) return;
+  float4 v[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+    v[q] = *reinterpret_cast<const float4*>(src + (2 * w0 + 1) * SLOT + q * 4 * (2 * TM));
+  for (int c = w0 + 1; c <= w1; ++c) {
+    float4 e[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) e[q] = *reinterpret_cast<const float4*>(src + 2 * c * SLOT + q * 4 * (2 * TM));
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      v[q].x += e[q].x;
+      v[q].y += e[q].y;
+      v[q].z += e[q].z;
+      v[q].w += e[q].w;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    if (oq + q * 4 >= a.n_out) break;
+    float* d = a.dW + (oq + q * 4) * a.ldw + i;
+    const float r[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+    if (a.vec_out && !a.accumulate && i + 4 <= a.n_in) {
+      *reinterpret_cast<float4*>(d) = v[q];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < a.n_in) d[k] = a.accumulate ? d[k] + r[k] : r[k];
+    }
   }
 }
 
@@ -601,61 +655,94 @@ __device__ __forceinline__ void split3(float x, float (&t)[3]) {
   t[2] = r - t[1];
 }
 
+// ... a thread takes 8 neighbouring columns.
 template <typename TD>
-__global__ void __launch_bounds__(256) terms_kernel(const TD* delta, int64_t ldd, bool vec, int64_t rows, int64_t n,
+__global__ void __launch_bounds__(256) terms_kernel(const TD* delta, int64_t ldd, bool vec, int64_t rows, int n,
                                                     __nv_bfloat16* out, int64_t ldo) {
   const int64_t upr = ldo / 8, total = rows * upr;
   for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < total; u += gridDim.x * 256ll) {
-    const int64_t r = u / upr, c = (u - r * upr) * 8;
-    float v[8];
-    load8(delta + r * ldd, c, n, vec, v);
-    __nv_bfloat16* d = out + r * ldo;
-    if (sizeof(TD) == 2) {
-      store8(d, c, ldo, true, v);
-    } else {
-      float t[3][8];
+    const int64_t r = u / upr;
+    const int c = (int)(u - r * upr) * 8;
+    const TD* row = delta + r * ldd;
+    __nv_bfloat16* d = out + r * ldo + c;
+    float t[3][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float e[3];
-        split3(v[i], e);
-        t[0][i] = e[0];
-        t[1][i] = e[1];
-        t[2][i] = e[2];
+    for (int h = 0; h < 8; h += 4) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (vec) {
+        unpack(load_raw<TD, 4>(row, c + h, n), v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + h + i < n) v[i] = ld_elem(row, c + h + i);
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q) store8(d + q * rows * ldo, c, ldo, true, t[q]);
+      for (int i = 0; i < 4; ++i) {
+        if (sizeof(TD) == 2) {
+          t[0][h + i] = v[i];
+        } else {
+          float e[3];
+          split3(v[i], e);
+          t[0][h + i] = e[0];
+          t[1][h + i] = e[1];
+          t[2][h + i] = e[2];
+        }
+      }
     }
+#pragma unroll
+    for (int q = 0; q < (sizeof(TD) == 2 ? 1 : 3); ++q) store_vec<8, true>(d + q * rows * ldo, 0, 8, t[q]);
   }
 }
 
-// Sums over a share of the rows of 256 columns, 8 a lane; warps take every eighth row
-// of the share and are added in order.
-template <typename TD>
+// db: sums over a share of the rows of 32 V columns, V a lane; a warp takes every eighth row of the
+// share, four at a time, and the warps' sums are added in order.
+template <typename TD, int V>
 __global__ void __launch_bounds__(256)
-column_sums_kernel(const TD* d, int64_t ldd, bool vec, int64_t rows, int64_t n, float* part) {
-  __shared__ float sum[256];
+column_sums_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part) {
+  __shared__ float sum[32 * V];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int64_t r = (int64_t)blockIdx.y * 8 + wp; r < rows; r += (int64_t)gridDim.y * 8) {
-    float v[8];
-    load8(d + r * ldd, c, n, vec, v);
+  const int c = blockIdx.x * 32 * V + lane * V;
+  float s[V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] += v[i];
+  for (int i = 0; i < V; ++i) s[i] = 0.f;
+  const int64_t stride = (int64_t)gridDim.y * 8;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + wp; r < rows; r += 4 * stride) {
+    Raw<TD, V> q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      memset(&q[j], 0, sizeof(q[j]));
+      if (r + j * stride < rows) q[j] = load_raw<TD, V>(d + (r + j * stride) * ldd, c, n);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[V];
+      unpack(q[j], v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += v[i];
+    }
   }
   for (int q = 0; q < 8; ++q) {
     __syncthreads();
     if (q != wp) continue;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[lane * 8 + i] = q == 0 ? s[i] : sum[lane * 8 + i] + s[i];
+    for (int i = 0; i < V; ++i) sum[lane * V + i] = q == 0 ? s[i] : sum[lane * V + i] + s[i];
   }
   __syncthreads();
-  const int64_t cc = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (cc < n) part[(int64_t)blockIdx.y * n + cc] = sum[threadIdx.x];
+  for (int k = threadIdx.x; k < 32 * V; k += 256) {
+    const int cc = blockIdx.x * 32 * V + k;
+    if (cc < n) part[(int64_t)blockIdx.y * n + cc] = sum[k];
+  }
 }
 
+// Shares of the rows: enough blocks of 256 columns to fill the GPU four times, 64 rows a share at least.
 int64_t sum_splits(int64_t rows, int64_t n) {
-  return mx<int64_t>(1, mn<int64_t>(cdiv(rows, 64), 148 * 4 / cdiv(n, 256)));
+  return std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, 64), SM_COUNT * 4 / cdiv(n, 256)));
+}
+
+template <typename TD, int V>
+void column_sums(const TD* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part, cudaStream_t s) {
+  column_sums_kernel<TD, V><<<dim3((unsigned)cdiv(n, 32 * V), (unsigned)splits), 256, 0, s>>>(d, ldd, rows, (int)n,
+                                                                                           part);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -732,7 +819,8 @@ bool codes_map(CUtensorMap* m, const int8_t* c, int64_t ld, int64_t rows, int64_
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, cudaStream_t s) {
+int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const float* sums, int parts, float* db,
+           cudaStream_t s) {
   static thread_local int done_dev = -1;
   int dev = 0;
   IFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -752,7 +840,9 @@ int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, cudaStre
   cfg.attrs = at;
   cfg.numAttrs = 1;
   IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel, dm, cm, a));
-  if (a.p.total) join_kernel<<<dim3((unsigned)(a.p.total / a.p.Kt), TN / 16), 2 * TM, 0, s>>>(a);
+  const int64_t joins = a.p.total && a.p.Gs > 1 ? a.p.total / a.p.Kt * (TN / JOIN_COLS) : 0;
+  const int64_t blocks = joins + (db ? cdiv(a.n_out, 32) : 0);
+  if (blocks) finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(a, (int)joins, sums, parts, db);
   IFK_CUDA_TRY(cudaGetLastError());
   return IFK_OK;
 }
@@ -763,7 +853,7 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
         uint8_t* ws, cudaStream_t s) {
   if (!encoder()) return IFK_ERR_CUDA;
   const int dtype = sizeof(TD) == 2 ? IFK_BF16 : IFK_F32;
-  const Layout l = layout(rows, n_out, n_in, dtype, !rows_aligned(delta, ldd));
+  const Layout l = layout(rows, n_out, n_in, dtype, !rows_allow<TD>(delta, ldd, 8));
   float* sums = (float*)ws;
   __nv_bfloat16* terms = (__nv_bfloat16*)(ws + l.sums);
   Args a;
@@ -778,14 +868,15 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.dW = dW;
   a.part = (float*)(ws + l.sums + l.terms_b);
   a.accumulate = accumulate;
+  a.vec_out = ((uintptr_t)dW & 15) == 0 && ldw % 4 == 0;
   a.vec_scales = ((uintptr_t)scales & 3) == 0 && lds % 4 == 0;
   a.status = status;
   const void* src = delta;
   int64_t ld = ldd;
   if (l.copy) {
     const int64_t g = cdiv(rows * (l.ldo / 8), 256);
-    terms_kernel<TD><<<(unsigned)mn<int64_t>(g, SM_COUNT * 16), 256, 0, s>>>(delta, ldd, rows_aligned(delta, ldd), rows,
-                                                                            n_out, terms, l.ldo);
+    terms_kernel<TD><<<(unsigned)mn<int64_t>(g, SM_COUNT * 16), 256, 0, s>>>(delta, ldd, rows_allow<TD>(delta, ldd, 4), rows,
+                                                                            (int)n_out, terms, l.ldo);
     IFK_CUDA_TRY(cudaGetLastError());
     src = terms;
     ld = l.ldo;
@@ -794,13 +885,14 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.whole = n_out % 64 == 0;
   if (!delta_map(&dm, src, ld, rows, n_out, l.terms, a.whole) || !codes_map(&cm, codes, ldc, rows, n_in))
     return IFK_ERR_SHAPE;
-  const int rc = launch(dm, cm, a, s);
-  if (rc != IFK_OK || !db) return rc;
-  const int64_t parts = sum_splits(rows, n_out);
-  column_sums_kernel<TD><<<dim3((unsigned)cdiv(n_out, 256), (unsigned)parts), 256, 0, s>>>(
-      delta, ldd, rows_aligned(delta, ldd), rows, n_out, sums);
-  IFK_CUDA_TRY(cudaGetLastError());
-  return sum_parts_run(sums, parts, n_out, db, nullptr, nullptr, accumulate, s);
+  const int parts = (int)sum_splits(rows, n_out);
+  if (db) {
+    constexpr int V = 16 / sizeof(TD);
+    if (rows_allow<TD>(delta, ldd, V)) column_sums<TD, V>(delta, ldd, rows, n_out, parts, sums, s);
+    else column_sums<TD, 1>(delta, ldd, rows, n_out, parts, sums, s);
+    IFK_CUDA_TRY(cudaGetLastError());
+  }
+  return launch(dm, cm, a, sums, parts, db, s);
 }
 
 }  // namespace
