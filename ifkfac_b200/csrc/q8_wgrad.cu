@@ -655,50 +655,13 @@ __device__ __forceinline__ void split3(float x, float (&t)[3]) {
   t[2] = r - t[1];
 }
 
-// ... a thread takes 8 neighbouring columns.
-template <typename TD>
-__global__ void __launch_bounds__(256) terms_kernel(const TD* delta, int64_t ldd, bool vec, int64_t rows, int n,
-                                                    __nv_bfloat16* out, int64_t ldo) {
-  const int64_t upr = ldo / 8, total = rows * upr;
-  for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < total; u += gridDim.x * 256ll) {
-    const int64_t r = u / upr;
-    const int c = (int)(u - r * upr) * 8;
-    const TD* row = delta + r * ldd;
-    __nv_bfloat16* d = out + r * ldo + c;
-    float t[3][8];
-#pragma unroll
-    for (int h = 0; h < 8; h += 4) {
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (vec) {
-        unpack(load_raw<TD, 4>(row, c + h, n), v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + h + i < n) v[i] = ld_elem(row, c + h + i);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (sizeof(TD) == 2) {
-          t[0][h + i] = v[i];
-        } else {
-          float e[3];
-          split3(v[i], e);
-          t[0][h + i] = e[0];
-          t[1][h + i] = e[1];
-          t[2][h + i] = e[2];
-        }
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < (sizeof(TD) == 2 ? 1 : 3); ++q) store_vec<8, true>(d + q * rows * ldo, 0, 8, t[q]);
-  }
-}
-
-// db: sums over a share of the rows of 32 V columns, V a lane; a warp takes every eighth row of the
-// share, four at a time, and the warps' sums are added in order.
-template <typename TD, int V>
+// One pass over delta before the products, by blocks of 32 V columns, V a lane, over a share of the
+// rows: a warp takes every eighth row of the share, four at a time.  part: the shares' column sums (db;
+// the warps' sums are added in order), or null.  TERMS: delta's bf16 terms go to `out` (rows x ldo
+// each, 16-byte aligned rows, columns past n as 0).
+template <typename TD, int V, bool TERMS>
 __global__ void __launch_bounds__(256)
-column_sums_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part) {
+delta_pass_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part, __nv_bfloat16* out, int64_t ldo) {
   __shared__ float sum[32 * V];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 * V + lane * V;
@@ -719,8 +682,27 @@ column_sums_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part) {
       unpack(q[j], v);
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] += v[i];
+      if (TERMS && r + j * stride < rows && c < ldo) {
+        __nv_bfloat16* o = out + (r + j * stride) * ldo + c;
+        if constexpr (sizeof(TD) == 2) {
+          store_vec<V, true>(o, 0, V, v);
+        } else {
+          float t[3][V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float e[3];
+            split3(v[i], e);
+            t[0][i] = e[0];
+            t[1][i] = e[1];
+            t[2][i] = e[2];
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) store_vec<V, true>(o + k * rows * ldo, 0, V, t[k]);
+        }
+      }
     }
   }
+  if (!part) return;
   for (int q = 0; q < 8; ++q) {
     __syncthreads();
     if (q != wp) continue;
@@ -739,17 +721,23 @@ int64_t sum_splits(int64_t rows, int64_t n) {
   return std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, 64), SM_COUNT * 4 / cdiv(n, 256)));
 }
 
-template <typename TD, int V>
-void column_sums(const TD* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part, cudaStream_t s) {
-  column_sums_kernel<TD, V><<<dim3((unsigned)cdiv(n, 32 * V), (unsigned)splits), 256, 0, s>>>(d, ldd, rows, (int)n,
-                                                                                           part);
+template <typename TD, bool TERMS>
+void delta_pass(const TD* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part, __nv_bfloat16* out,
+                int64_t ldo, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(TD);
+  if (rows_allow<TD>(d, ldd, V))
+    delta_pass_kernel<TD, V, TERMS><<<dim3((unsigned)cdiv(TERMS ? ldo : n, 32 * V), (unsigned)splits), 256, 0, s>>>(
+        d, ldd, rows, (int)n, part, out, ldo);
+  else
+    delta_pass_kernel<TD, 1, TERMS><<<dim3((unsigned)cdiv(TERMS ? ldo : n, 32), (unsigned)splits), 256, 0, s>>>(
+        d, ldd, rows, (int)n, part, out, ldo);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Host side of one call: sizes of the workspace parts and the division of the work.
 struct Layout {
-  bool copy;           // delta goes through terms_kernel
+  bool copy;           // the products read delta's terms in the workspace, not delta
   int terms;
   int64_t ldo;         // pitch of the copied terms
   size_t sums, terms_b, part;
@@ -773,7 +761,7 @@ Plan make_plan(int64_t rows, int64_t n_out, int64_t n_in, int terms) {
 Layout layout(int64_t rows, int64_t n_out, int64_t n_in, int dtype, bool copy) {
   Layout l;
   l.terms = dtype == IFK_F32 ? 3 : 1;
-  l.copy = copy || dtype == IFK_F32;
+  l.copy = copy || dtype == IFK_F32;  // three terms, or rows that TMA cannot read
   l.ldo = cdiv(n_out, 8) * 8;
   l.sums = up256((size_t)sum_splits(rows, n_out) * (size_t)n_out * sizeof(float));
   l.terms_b = l.copy ? up256((size_t)l.terms * (size_t)rows * (size_t)l.ldo * 2) : 0;
@@ -871,27 +859,22 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.vec_out = ((uintptr_t)dW & 15) == 0 && ldw % 4 == 0;
   a.vec_scales = ((uintptr_t)scales & 3) == 0 && lds % 4 == 0;
   a.status = status;
+  const int parts = (int)sum_splits(rows, n_out);
   const void* src = delta;
   int64_t ld = ldd;
   if (l.copy) {
-    const int64_t g = cdiv(rows * (l.ldo / 8), 256);
-    terms_kernel<TD><<<(unsigned)mn<int64_t>(g, SM_COUNT * 16), 256, 0, s>>>(delta, ldd, rows_allow<TD>(delta, ldd, 4), rows,
-                                                                            (int)n_out, terms, l.ldo);
+    delta_pass<TD, true>(delta, ldd, rows, n_out, parts, db ? sums : nullptr, terms, l.ldo, s);
     IFK_CUDA_TRY(cudaGetLastError());
     src = terms;
     ld = l.ldo;
+  } else if (db) {
+    delta_pass<TD, false>(delta, ldd, rows, n_out, parts, sums, nullptr, 0, s);
+    IFK_CUDA_TRY(cudaGetLastError());
   }
   CUtensorMap dm, cm;
   a.whole = n_out % 64 == 0;
   if (!delta_map(&dm, src, ld, rows, n_out, l.terms, a.whole) || !codes_map(&cm, codes, ldc, rows, n_in))
     return IFK_ERR_SHAPE;
-  const int parts = (int)sum_splits(rows, n_out);
-  if (db) {
-    constexpr int V = 16 / sizeof(TD);
-    if (rows_allow<TD>(delta, ldd, V)) column_sums<TD, V>(delta, ldd, rows, n_out, parts, sums, s);
-    else column_sums<TD, 1>(delta, ldd, rows, n_out, parts, sums, s);
-    IFK_CUDA_TRY(cudaGetLastError());
-  }
   return launch(dm, cm, a, sums, parts, db, s);
 }
 
