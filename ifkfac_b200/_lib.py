@@ -77,7 +77,7 @@ SIGNATURES = {
                              _i64, _vp, _i64, _vp]),
     "ifk_layernorm_backward_workspace": (_sz, [_i64, _i64]),
     "ifk_layernorm_backward": (_int, [_vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _int,
-                                      _i64, _i64, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
+                                      _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -314,11 +314,12 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
 
 
 def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optional[torch.Tensor] = None,
-                        weight_grads: bool = True
+                        weight_grads: bool = True, status: Optional[torch.Tensor] = None
                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw, db) of :func:`layer_norm_forward`: dx in the input's dtype, dw and db
-    fp32 (None without ``weight_grads``)."""
-    dev = _need_cuda(dy, saved.stats, weight)
+    fp32 (None without ``weight_grads``).  ``status`` (a device int32, optional)
+    receives IFK_ERR_TIMEOUT if a wait on the device gave up."""
+    dev = _need_cuda(dy, saved.stats, weight, status)
     dy, rows, n, ld = _rows2d(dy, "dy")
     dt, xdt = _code(dy.dtype), _code(saved.x_dtype)
     if rows != saved.rows or n != saved.cols:
@@ -338,7 +339,7 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     mean = saved.stats.data_ptr()
     _call("ifk_layernorm_backward", dev, dy.data_ptr(), ld, dt, x, ldx, xdt, *q, mean, mean + 4 * rows, _ptr(weight),
-          wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+          wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(status), _ptr(ws), nbytes)
     return dx, dw, db
 
 

@@ -75,12 +75,20 @@ __device__ __forceinline__ void write_out(const FwdArgs& a, TY* y, int c, const 
   if constexpr (PLAIN) {
     load_f32<V>((const float*)a.w, c, w);
     load_f32<V>((const float*)a.b, c, b);
+    F2 q[V / 2], w2[V / 2], b2[V / 2];
+    pairs(v, q);
+    pairs(w, w2);
+    pairs(b, b2);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      q[i] = fma2(mul(add(add(q[i], f2(-t.m1)), f2(-t.c1)), f2(t.rstd)), w2[i], b2[i]);
+    singles(q, o);
   } else {
     load_param<V>(a.w, a.w_bf16, 1.f, c, a.n, w);
     load_param<V>(a.b, a.w_bf16, 0.f, c, a.n, b);
-  }
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = fmaf((v[i] - t.m1 - t.c1) * t.rstd, w[i], b[i]);
+    for (int i = 0; i < V; ++i) o[i] = fmaf((v[i] - t.m1 - t.c1) * t.rstd, w[i], b[i]);
+  }
   store_vec<V, PLAIN>(y, c, a.n, o);
 }
 
@@ -98,26 +106,66 @@ __global__ void __launch_bounds__(512, 2) forward_kernel(const FwdArgs a) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) r[k] = load_raw<TX, V, PLAIN>(x, c0 + k * step, a.n);
   float s = 0.f, sd = 0.f, sd2 = 0.f;
+  if constexpr (PLAIN) {
+    F2 s2 = f2(0.f);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    float v[V];
-    unpack(r[k], v);
+    for (int k = 0; k < NV; ++k) {
+      float v[V];
+      F2 q[V / 2];
+      unpack(r[k], v);
+      pairs(v, q);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += v[i];
+      for (int i = 0; i < V / 2; ++i) s2 = add(s2, q[i]);
+    }
+    s = sum(s2);
+  } else {
+    // even and odd columns apart, as the pairs of the plain form: the same bits
+    float odd = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float v[V];
+      unpack(r[k], v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) (i & 1 ? odd : s) += v[i];
+    }
+    s += odd;
   }
   const float m1 = team_sum(s, W, buf[0]) * inv_n;
+  if constexpr (PLAIN) {
+    F2 d1 = f2(0.f), d2 = f2(0.f);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = c0 + k * step;
-    if (c >= a.n) continue;
-    float v[V];
-    unpack(r[k], v);
+    for (int k = 0; k < NV; ++k) {
+      if (c0 + k * step >= a.n) continue;
+      float v[V];
+      F2 q[V / 2];
+      unpack(r[k], v);
+      pairs(v, q);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = PLAIN || c + i < a.n ? v[i] - m1 : 0.f;
-      sd += d;
-      sd2 = fmaf(d, d, sd2);
+      for (int i = 0; i < V / 2; ++i) {
+        const F2 d = add(q[i], f2(-m1));
+        d1 = add(d1, d);
+        d2 = fma2(d, d, d2);
+      }
     }
+    sd = sum(d1);
+    sd2 = sum(d2);
+  } else {
+    float odd = 0.f, odd2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      float v[V];
+      unpack(r[k], v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = c + i < a.n ? v[i] - m1 : 0.f;
+        (i & 1 ? odd : sd) += d;
+        float& q = i & 1 ? odd2 : sd2;
+        q = fmaf(d, d, q);
+      }
+    }
+    sd += odd;
+    sd2 += odd2;
   }
   sd = warp_sum(sd);
   sd2 = warp_sum(sd2);

@@ -1,16 +1,19 @@
 // Layer norm, backward (ifk_layernorm_backward): dx, and the sums over the rows dw, db.
 //
 // Bound by memory: dy and the saved rows (as they were, or in 8 bits) are read once, dx
-// is written once.  A team of W warps holds a row, 16 columns a lane; the teams of a
-// persistent block walk the rows, each lane with the sums of its own 16 columns for dw
-// and db in registers and the next row's loads in flight.  At the end the block adds its
-// teams' sums in shared memory and writes one row of partial sums; a second kernel adds
-// the blocks'.  The order of every sum is fixed by the sizes.
+// is written once.  A team of W warps holds a row, COLS columns a lane; the teams of a
+// persistent block walk the rows, each lane with the sums of its own columns for dw and
+// db in registers, and a ring of rows in shared memory a team, that bulk copies keep
+// filled.  At the end the block adds its teams' sums in shared memory and writes one row
+// of partial sums; a second kernel adds the blocks'.  The order of every sum is fixed by
+// the sizes.  fp32 arithmetic goes two to an instruction (F2): the instructions, not the
+// memory, bound a row of 768 columns in 8 bits otherwise.
 #include <algorithm>
 #include <cstring>
 
 #include "rowvec.cuh"
 #include "ifk_internal.h"
+#include "pipe.cuh"
 
 namespace ifk {
 
@@ -29,147 +32,42 @@ struct BwdArgs {
   int64_t lddy, ldx, ldc, lds, lddx, rows;
   int n;
   bool w_bf16;
-  int W, teams;  // warps a row, teams a block
+  int W, teams, depth;  // warps a row, teams a block, rows of a team's ring
+  int* status;
 };
 
-constexpr int COLS = 16;       // columns a lane holds
-constexpr int MAX_W = 16;      // warps a row: up to 32 * 16 * COLS = 8192 columns
-constexpr int BLOCK_WARPS = 16;
+// A lane holds 32 columns of a row of up to 1024 columns (one warp, no barrier), else 16.
+constexpr int NARROW = 1024;
+constexpr int MAX_W = 16;  // warps a row: up to 32 * 16 * 16 = 8192 columns
+template <int COLS>
+constexpr int block_warps() { return COLS == 32 ? 12 : 16; }  // 168 or 128 registers a thread
 
-// A barrier of one team's warps.
-__device__ __forceinline__ void team_barrier(int team, int W) {
-  asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(W * 32) : "memory");
-}
-
-// What a lane reads of a row.
-template <typename TX, typename TY, int V, bool Q8, bool PLAIN>
-struct RowIn {
-  static constexpr int NV = COLS / V;
-  Raw<TY, V> dy[NV];
-  Raw<TX, V> x[Q8 ? 1 : NV];
-  q8::Codes<V> c[Q8 ? NV : 1];
-  uint8_t s[Q8 ? NV : 1];
-  float mean, rstd;
-  __device__ __forceinline__ void load(const BwdArgs& a, int64_t row, int c0, int step) {
-    mean = a.mean[row];
-    rstd = a.rstd[row];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = c0 + k * step;
-      dy[k] = load_raw<TY, V, PLAIN>((const TY*)a.dy + row * a.lddy, col, a.n);
-      if (Q8) {
-        if (col < a.n) {
-          c[k % (Q8 ? NV : 1)] = q8::load_codes<V>(a.codes + row * a.ldc + col);
-          s[k % (Q8 ? NV : 1)] = a.scales[row * a.lds + col / q8::GROUP];
-        } else {
-          c[k % (Q8 ? NV : 1)] = q8::Codes<V>{};
-          s[k % (Q8 ? NV : 1)] = 0;
-        }
-      } else {
-        x[k % (Q8 ? 1 : NV)] = load_raw<TX, V, PLAIN>((const TX*)a.x + row * a.ldx, col, a.n);
-      }
-    }
-  }
-  // the saved values of access k
-  __device__ __forceinline__ void saved(int k, float (&v)[V]) const {
-    if (Q8) q8::values<V>(c[k % (Q8 ? NV : 1)], q8::scale_of(s[k % (Q8 ? NV : 1)]), v);
-    else unpack(x[k % (Q8 ? 1 : NV)], v);
-  }
-};
-
-// PLAIN: n is a multiple of V, w is there and fp32.
-template <typename TX, typename TY, int V, bool Q8, bool PLAIN>
-__global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_kernel(const BwdArgs a) {
-  using In = RowIn<TX, TY, V, Q8, PLAIN>;
-  constexpr int NV = In::NV;
-  __shared__ float2 buf[2][BLOCK_WARPS];
-  extern __shared__ float sums[];  // n, with several teams
-  const int W = a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int team = warp / W;
-  const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
-  const float inv_n = 1.f / (float)a.n;
-  const int64_t stride = (int64_t)gridDim.x * a.teams;
-  float sw[NV][V], sb[NV][V];
+// The block's sums over its rows: the teams' go to shared memory (2 n floats a team) and are added in order.
+template <int V, int NV>
+__device__ __forceinline__ void write_sums(const BwdArgs& a, int team, int c0, int step, const float (&sw)[NV][V],
+                                           const float (&sb)[NV][V], float* sums) {
+  __syncthreads();
+  float* mine = sums + (size_t)team * 2 * a.n;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) sw[k][i] = sb[k][i] = 0.f;
-  int64_t row = (int64_t)blockIdx.x * a.teams + team;
-  In in;
-  if (row < a.rows) in.load(a, row, c0, step);
-  for (int par = 0; row < a.rows; row += stride, par ^= 1) {
-    // (one element an access, the unaligned case, has no registers left for a row ahead)
-    In next;
-    if (V > 1 && row + stride < a.rows) next.load(a, row + stride, c0, step);
-    float g[NV][V], z[NV][V];
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * step;
-      unpack(in.dy[k], g[k]);
-      if (PLAIN && c >= a.n) continue;  // dy is 0 there
-      float w[V];
-      if constexpr (PLAIN) load_f32<V>((const float*)a.w, c, w);
-      else load_param<V>(a.w, a.w_bf16, 1.f, c, a.n, w);
-      in.saved(k, z[k]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        z[k][i] = PLAIN || c + i < a.n ? (z[k][i] - in.mean) * in.rstd : 0.f;
-        sw[k][i] = fmaf(g[k][i], z[k][i], sw[k][i]);
-        sb[k][i] += g[k][i];
-        g[k][i] = PLAIN || c + i < a.n ? g[k][i] * w[i] : 0.f;
-        s.x += g[k][i];
-        s.y = fmaf(g[k][i], z[k][i], s.y);
-      }
-    }
-    s.x = warp_sum(s.x);
-    s.y = warp_sum(s.y);
-    if (W > 1) {
-      // two buffers in turn: the barrier of the next row stands between its writes and these reads
-      if (lane == 0) buf[par][warp] = s;
-      team_barrier(team, W);
-      s = make_float2(0.f, 0.f);
-      for (int i = 0; i < W; ++i) {
-        const float2 q = buf[par][team * W + i];
-        s.x += q.x;
-        s.y += q.y;
-      }
-    }
-    const float m1 = s.x * inv_n * in.rstd, m2 = s.y * inv_n * in.rstd;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * step;
+    for (int i = 0; i < V; ++i) {
+      const int c = c0 + k * step + i;
       if (c >= a.n) continue;
-      float o[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fmaf(in.rstd, g[k][i], fmaf(-m2, z[k][i], -m1));
-      store_vec<V, PLAIN>((TX*)a.dx + row * a.lddx, c, a.n, o);
+      mine[c] = sw[k][i];
+      mine[a.n + c] = sb[k][i];
     }
-    if (V > 1) in = next;
-    else if (row + stride < a.rows) in.load(a, row + stride, c0, step);
-  }
-  if (!a.part) return;
-  for (int which = 0; which < 2; ++which) {
-    float* out = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.n;
-    for (int q = 0; q < a.teams; ++q) {
-      __syncthreads();
-      if (q != team) continue;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = c0 + k * step + i;
-          if (c >= a.n) continue;
-          float v = which ? sb[k][i] : sw[k][i];
-          if (q > 0) v += sums[c];
-          if (q + 1 < a.teams) sums[c] = v;
-          else out[c] = v;
-        }
-    }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.n; c += blockDim.x) {
+    float v = sums[c];
+    for (int q = 1; q < a.teams; ++q) v += sums[(size_t)q * 2 * a.n + c];
+    const int which = c >= a.n;
+    a.part[((int64_t)which * gridDim.x + blockIdx.x) * a.n + (c - which * a.n)] = v;
   }
 }
+size_t sums_bytes(const BwdArgs& a) { return a.part ? (size_t)a.teams * 2 * a.n * sizeof(float) : 0; }
 
-// Rows too wide for registers: dx by a block that walks its row twice ...
+// The values of a row that a thread works on: dy, and the saved row normalised; 0 past the end.
 template <typename TX, typename TY, int V, bool Q8>
 __device__ __forceinline__ void row_part(const BwdArgs& a, int64_t row, int c, float mean, float rstd, float (&g)[V],
                                          float (&z)[V]) {
@@ -184,6 +82,209 @@ __device__ __forceinline__ void row_part(const BwdArgs& a, int64_t row, int c, f
   for (int i = 0; i < V; ++i) z[i] = c + i < a.n ? (z[i] - mean) * rstd : 0.f;
 }
 
+// Rows straight from memory: any alignment and width.
+template <typename TX, typename TY, int V, bool Q8>
+__global__ void __launch_bounds__(512, 1) backward_kernel(const BwdArgs a) {
+  constexpr int NV = 16 / V;
+  __shared__ float2 buf[2][16];
+  extern __shared__ float sums[];
+  const int W = a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
+  const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
+  const float inv_n = 1.f / (float)a.n;
+  const int64_t stride = (int64_t)gridDim.x * a.teams;
+  float sw[NV][V], sb[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) sw[k][i] = sb[k][i] = 0.f;
+  int par = 0;
+  for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += stride, par ^= 1) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float g[NV][V], z[NV][V];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) row_part<TX, TY, V, Q8>(a, row, c0 + k * step, mean, rstd, g[k], z[k]);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      float w[V];
+      load_param<V>(a.w, a.w_bf16, 1.f, c, a.n, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        sw[k][i] = fmaf(g[k][i], z[k][i], sw[k][i]);
+        sb[k][i] += g[k][i];
+        g[k][i] = c + i < a.n ? g[k][i] * w[i] : 0.f;
+        s.x += g[k][i];
+        s.y = fmaf(g[k][i], z[k][i], s.y);
+      }
+    }
+    s.x = warp_sum(s.x);
+    s.y = warp_sum(s.y);
+    if (W > 1) {
+      // two buffers in turn: the barrier of the next row stands between its writes and these reads
+      if (lane == 0) buf[par][warp] = s;
+      named_barrier(team + 1, W * 32);
+      s = make_float2(0.f, 0.f);
+      for (int i = 0; i < W; ++i) {
+        const float2 q = buf[par][team * W + i];
+        s.x += q.x;
+        s.y += q.y;
+      }
+    }
+    const float m1 = s.x * inv_n * rstd, m2 = s.y * inv_n * rstd;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      if (c >= a.n) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, g[k][i], fmaf(-m2, z[k][i], -m1));
+      store_vec<V>((TX*)a.dx + row * a.lddx, c, a.n, o);
+    }
+  }
+  if (a.part) write_sums<V, NV>(a, team, c0, step, sw, sb, sums);
+}
+
+// Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
+// A wait that gives up marks the call and the block goes on (its result is not valid).
+template <typename TX, typename TY, int V, int COLS, bool Q8>
+__global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_kernel(const BwdArgs a) {
+  constexpr int NV = COLS / V, H = V / 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 buf[2][16];
+  __shared__ int failed;
+  const int W = a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
+  const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
+  const bool leader = lane == 0 && warp == team * W;
+  const int dy_bytes = a.n * (int)sizeof(TY);
+  const int x_bytes = Q8 ? (int)q8::pitch(a.n) : a.n * (int)sizeof(TX), bytes = dy_bytes + x_bytes;
+  uint8_t* ring = smem + (size_t)team * a.depth * bytes;
+  const uint32_t data = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t full = (uint32_t)__cvta_generic_to_shared(smem + (size_t)a.teams * a.depth * bytes) +
+                        (uint32_t)(team * a.depth * 8);
+  const int64_t stride = (int64_t)gridDim.x * a.teams, first = (int64_t)blockIdx.x * a.teams + team;
+  if (threadIdx.x == 0) failed = 0;
+  if (leader) {
+    for (int i = 0; i < a.depth; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  auto fetch = [&](int64_t row, int slot) {
+    const uint32_t bar = full + 8 * slot, dst = data + slot * bytes;
+    expect(bar, bytes);
+    bulk_load(dst, (const TY*)a.dy + row * a.lddy, dy_bytes, bar);
+    if (Q8) bulk_load(dst + dy_bytes, a.codes + row * a.ldc, x_bytes, bar);
+    else bulk_load(dst + dy_bytes, (const TX*)a.x + row * a.ldx, x_bytes, bar);
+  };
+  if (leader)
+    for (int i = 0; i < a.depth && first + i * stride < a.rows; ++i) fetch(first + i * stride, i);
+  const float inv_n = 1.f / (float)a.n;
+  const bool w_f32 = a.w && !a.w_bf16;
+  F2 sw[NV][H], sb[NV][H];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < H; ++i) sw[k][i] = sb[k][i] = f2(0.f);
+  // what is not in the ring, a row ahead: the statistics, and the scales of the 8-bit rows
+  float mean = 0.f, rstd = 0.f;
+  uint8_t sc[Q8 ? NV : 1];
+  auto ahead = [&](int64_t row) {
+    mean = a.mean[row];
+    rstd = a.rstd[row];
+    if (Q8) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = c0 + k * step;
+        sc[k % (Q8 ? NV : 1)] = c < a.n ? a.scales[row * a.lds + c / q8::GROUP] : 0;
+      }
+    }
+  };
+  if (first < a.rows) ahead(first);
+  int slot = 0, ph = 0, par = 0;
+  for (int64_t row = first; row < a.rows; row += stride, par ^= 1) {
+    const float mu = mean, rs = rstd;
+    uint8_t s8[Q8 ? NV : 1];
+#pragma unroll
+    for (int k = 0; k < (Q8 ? NV : 1); ++k) s8[k] = sc[k];
+    if (row + stride < a.rows) ahead(row + stride);
+    wait_bar(full + 8 * slot, ph, &failed);
+    const uint8_t* in = ring + (size_t)slot * bytes;
+    F2 g[NV][H], z[NV][H], sx = f2(0.f), sy = f2(0.f);
+    const F2 nmu = f2(-mu), rs2 = f2(rs);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      if (c >= a.n) continue;
+      float v[V];
+      unpack(shared_raw<TY, V>(in, c, a.n), v);
+      pairs(v, g[k]);
+      if constexpr (Q8) {
+        q8::values2<V>(q8::load_codes<V>((const int8_t*)in + dy_bytes + c), q8::scale_of(s8[k]), z[k]);
+      } else {
+        unpack(shared_raw<TX, V>(in + dy_bytes, c, a.n), v);
+        pairs(v, z[k]);
+      }
+      F2 w[H];
+      if (w_f32) load_f32<V>((const float*)a.w, c, v);
+      else load_param<V>(a.w, a.w_bf16, 1.f, c, a.n, v);
+      pairs(v, w);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        z[k][i] = mul(add(z[k][i], nmu), rs2);
+        sw[k][i] = fma2(g[k][i], z[k][i], sw[k][i]);
+        sb[k][i] = add(sb[k][i], g[k][i]);
+        g[k][i] = mul(g[k][i], w[i]);
+        sx = add(sx, g[k][i]);
+        sy = fma2(g[k][i], z[k][i], sy);
+      }
+    }
+    float2 s = make_float2(warp_sum(sum(sx)), warp_sum(sum(sy)));
+    if (W > 1) {
+      // two buffers in turn: the barrier of the next row stands between its writes and these reads
+      if (lane == 0) buf[par][warp] = s;
+      named_barrier(team + 1, W * 32);
+      s = make_float2(0.f, 0.f);
+      for (int i = 0; i < W; ++i) {
+        const float2 q = buf[par][team * W + i];
+        s.x += q.x;
+        s.y += q.y;
+      }
+    }
+    // every lane of the team has read the row
+    if (leader && row + a.depth * stride < a.rows) fetch(row + a.depth * stride, slot);
+    if (++slot == a.depth) {
+      slot = 0;
+      ph ^= 1;
+    }
+    const F2 m1 = f2(-s.x * inv_n * rs), m2 = f2(-s.y * inv_n * rs);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      if (c >= a.n) continue;
+      F2 q[H];
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < H; ++i) q[i] = fma2(rs2, g[k][i], fma2(m2, z[k][i], m1));
+      singles(q, o);
+      store_vec<V, true>((TX*)a.dx + row * a.lddx, c, a.n, o);
+    }
+  }
+  if (failed && leader) {
+    linger();
+    if (a.status) *a.status = IFK_ERR_TIMEOUT;
+  }
+  if (!a.part) return;
+  float w[NV][V], b[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    singles(sw[k], w[k]);
+    singles(sb[k], b[k]);
+  }
+  write_sums<V, NV>(a, team, c0, step, w, b, reinterpret_cast<float*>(smem));
+}
+
+// Rows too wide for registers: dx by a block that walks its row twice ...
 template <typename TX, typename TY, int V, bool Q8>
 __global__ void __launch_bounds__(512) backward_long_kernel(const BwdArgs a) {
   __shared__ float2 buf[16];
@@ -258,35 +359,70 @@ __global__ void __launch_bounds__(256) backward_long_sums_kernel(const BwdArgs a
   }
 }
 
-// Persistent blocks: one an SM, fewer when the rows do not fill them (the partial sums are
-// written and read once a block).
-int row_warps(int64_t n) { return (int)cdiv(n, 32 * COLS); }
-int block_teams(int64_t n) { return std::max(1, BLOCK_WARPS / row_warps(n)); }
+// Persistent blocks: one an SM, fewer when the rows do not fill them (a block's partial sums are written
+// and read once).  The number of blocks depends on the sizes alone: it is the number of partial sums.
+int row_warps(int64_t n) { return n <= NARROW ? 1 : (int)cdiv(n, 32 * 16); }
 int64_t parts_of(int64_t rows, int64_t n) {
   if (row_warps(n) > MAX_W) return std::min<int64_t>(cdiv(rows, 64), 32);
-  return std::min<int64_t>(cdiv(rows, block_teams(n)), 148);
+  const int teams = n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / row_warps(n));
+  return std::min<int64_t>(cdiv(rows, teams), 148);
+}
+
+constexpr size_t RING_BYTES = 200 * 1024;
+
+// Whether the rows can come by bulk copies; sets the ring's depth.
+template <typename TX, typename TY, int V, bool Q8>
+bool ring_ok(BwdArgs& a, size_t* row) {
+  const size_t dy = (size_t)a.n * sizeof(TY), x = Q8 ? (size_t)q8::pitch(a.n) : (size_t)a.n * sizeof(TX);
+  *row = dy + x;
+  a.depth = (int)std::min<size_t>(8, RING_BYTES / (a.teams * *row));
+  return V > 1 && a.n % V == 0 && a.depth >= 2 && dy % 16 == 0 && x % 16 == 0 &&
+         rows_allow<uint8_t>(a.dy, a.lddy * (int64_t)sizeof(TY), 16) &&
+         (Q8 || rows_allow<uint8_t>(a.x, a.ldx * (int64_t)sizeof(TX), 16));
+}
+
+template <typename K>
+int launch(K kernel, int* done_dev, unsigned blocks, unsigned threads, size_t smem, const BwdArgs& a, cudaStream_t s) {
+  int dev = 0;
+  IFK_CUDA_TRY(cudaGetDevice(&dev));
+  if (*done_dev != dev) {
+    IFK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_BYTES + 2048));
+    *done_dev = dev;
+  }
+  kernel<<<blocks, threads, smem, s>>>(a);
+  IFK_CUDA_TRY(cudaGetLastError());
+  return IFK_OK;
+}
+
+template <typename TX, typename TY, int V, int COLS, bool Q8>
+int launch_ring(const BwdArgs& a, unsigned blocks, size_t row, cudaStream_t s) {
+  static thread_local int done_dev = -1;
+  return launch(backward_ring_kernel<TX, TY, V, COLS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
+                std::max<size_t>(a.teams * a.depth * (row + 8), sums_bytes(a)), a, s);
 }
 
 template <typename TX, typename TY, int V, bool Q8>
 int backward(BwdArgs& a, cudaStream_t s) {
-  const int64_t parts = parts_of(a.rows, a.n);
+  const unsigned parts = (unsigned)parts_of(a.rows, a.n);
   a.W = row_warps(a.n);
   if (a.W > MAX_W) {
     backward_long_kernel<TX, TY, V, Q8><<<(unsigned)a.rows, 512, 0, s>>>(a);
     if (a.part)
-      backward_long_sums_kernel<TX, TY, V, Q8>
-          <<<dim3((unsigned)cdiv(a.n, 32 * V), (unsigned)parts), 256, 0, s>>>(a);
-  } else {
-    a.teams = block_teams(a.n);
-    const size_t smem = a.part && a.teams > 1 ? (size_t)a.n * sizeof(float) : 0;
-    const unsigned threads = 32 * a.W * a.teams;
-    if (V > 1 && a.n % V == 0 && a.w && !a.w_bf16)
-      backward_kernel<TX, TY, V, Q8, V != 1><<<(unsigned)parts, threads, smem, s>>>(a);
-    else
-      backward_kernel<TX, TY, V, Q8, false><<<(unsigned)parts, threads, smem, s>>>(a);
+      backward_long_sums_kernel<TX, TY, V, Q8><<<dim3((unsigned)cdiv(a.n, 32 * V), parts), 256, 0, s>>>(a);
+    IFK_CUDA_TRY(cudaGetLastError());
+    return IFK_OK;
   }
-  IFK_CUDA_TRY(cudaGetLastError());
-  return IFK_OK;
+  a.teams = a.n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / a.W);
+  if constexpr (V > 1) {
+    size_t row;
+    if (ring_ok<TX, TY, V, Q8>(a, &row))
+      return a.n <= NARROW ? launch_ring<TX, TY, V, 32, Q8>(a, parts, row, s)
+                           : launch_ring<TX, TY, V, 16, Q8>(a, parts, row, s);
+  }
+  a.W = (int)cdiv(a.n, 32 * 16);
+  a.teams = std::max(1, 16 / a.W);
+  static thread_local int done_dev = -1;
+  return launch(backward_kernel<TX, TY, V, Q8>, &done_dev, parts, 32 * a.W * a.teams, sums_bytes(a), a, s);
 }
 
 template <typename TX, typename TY>
@@ -335,7 +471,7 @@ size_t layernorm_backward_bytes(int64_t rows, int64_t n) {
 int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype,
                            const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const float* mean,
                            const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n, void* dx,
-                           int64_t lddx, float* dw, float* db, float* part, cudaStream_t s) {
+                           int64_t lddx, float* dw, float* db, float* part, int* status, cudaStream_t s) {
   BwdArgs a;
   a.dy = dy;
   a.x = x;
@@ -354,7 +490,8 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
   a.rows = rows;
   a.n = (int)n;
   a.w_bf16 = w_dtype == IFK_BF16;
-  a.teams = 1;
+  a.teams = a.depth = 1;
+  a.status = status;
   using B = __nv_bfloat16;
   int rc;
   if (x_dtype == IFK_F32) rc = y_dtype == IFK_F32 ? backward_any<float, float>(a, s) : backward_any<float, B>(a, s);

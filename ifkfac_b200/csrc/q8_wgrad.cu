@@ -32,6 +32,7 @@
 
 #include "rowvec.cuh"
 #include "ifk_internal.h"
+#include "pipe.cuh"
 #include "tc.cuh"
 
 namespace ifk {
@@ -163,56 +164,6 @@ struct Walk {
 
 // ---- PTX ----
 
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait: gives up after two seconds, or when another warp of the CTA has.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* failed) {
-  uint64_t t0 = 0;
-  for (uint32_t it = 0;; ++it) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((it & 63) == 63) {
-      if (*failed) return false;
-      const uint64_t t = now_ns();
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > 2000000000ull) {
-        *failed = 1;
-        return false;
-      }
-    }
-  }
-}
-
-// One arrival, and the bytes of the copies that the barrier's phase also waits for.
-__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Whether the phase has completed, without waiting.
-__device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done;
-}
 // The address of the same place in the pair's first CTA.
 __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
   uint32_t r;
@@ -221,11 +172,6 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// After a failed wait: stay until the copies in flight have landed (microseconds).
-__device__ __forceinline__ void linger() {
-  const uint64_t t0 = now_ns();
-  while (now_ns() - t0 < 1000000ull) __nanosleep(1000);
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(

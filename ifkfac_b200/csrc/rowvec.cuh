@@ -15,6 +15,50 @@ template <> struct Raw<__nv_bfloat16, 8> { uint4 r; };
 template <> struct Raw<__nv_bfloat16, 4> { uint2 r; };
 template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 r; };
 
+// Two fp32 values in a 64-bit register: one instruction does both, each rounded on its own.
+struct F2 {
+  uint64_t r;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 q;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(q.r) : "f"(a), "f"(b));
+  return q;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ void split(F2 q, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(q.r));
+}
+__device__ __forceinline__ float sum(F2 q) {
+  float a, b;
+  split(q, a, b);
+  return a + b;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  F2 q;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(q.r) : "l"(a.r), "l"(b.r));
+  return q;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 q;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q.r) : "l"(a.r), "l"(b.r));
+  return q;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 q;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(q.r) : "l"(a.r), "l"(b.r), "l"(c.r));
+  return q;
+}
+template <int N>
+__device__ __forceinline__ void pairs(const float (&v)[2 * N], F2 (&q)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = f2(v[2 * i], v[2 * i + 1]);
+}
+template <int N>
+__device__ __forceinline__ void singles(const F2 (&q)[N], float (&v)[2 * N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) split(q[i], v[2 * i], v[2 * i + 1]);
+}
+
 __device__ __forceinline__ void bf16x2(uint32_t w, float& a, float& b) {
   a = __uint_as_float(w << 16);
   b = __uint_as_float(w & 0xffff0000u);
@@ -62,6 +106,15 @@ __device__ __forceinline__ Raw<T, V> load_raw(const T* row, int c, int n) {
     if (c + i < n) e[i] = row[c + i];
   }
   memcpy(&q, e, sizeof(q));
+  return q;
+}
+
+// The same columns of a row in shared memory; n is a multiple of V.
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> shared_raw(const uint8_t* row, int c, int n) {
+  Raw<T, V> q;
+  memset(&q, 0, sizeof(q));
+  if (c < n) q = *reinterpret_cast<const Raw<T, V>*>(row + (size_t)c * sizeof(T));
   return q;
 }
 
@@ -191,6 +244,17 @@ __device__ __forceinline__ Codes<V> load_codes(const int8_t* p) {
     c.w[0] = (uint8_t)*p;
   }
   return c;
+}
+template <int V>
+__device__ __forceinline__ void values2(const Codes<V>& c, float scale, F2 (&v)[V / 2]) {
+  const F2 s = f2(scale), off = f2(-8388736.f);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const uint32_t w = c.w[i / 2] ^ 0x80808080u;
+    const float a = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | (2 * i & 3)));
+    const float b = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | ((2 * i + 1) & 3)));
+    v[i] = mul(add(f2(a, b), off), s);
+  }
 }
 template <int V>
 __device__ __forceinline__ void values(const Codes<V>& c, float scale, float (&v)[V]) {

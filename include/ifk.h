@@ -553,14 +553,15 @@ IFK_API size_t ifk_layernorm_backward_workspace(int64_t rows, int64_t n);
  *   dw = sum over rows of dy z, db = sum over rows of dy   (n fp32; each may be NULL).
  * x (x_dtype) is the saved input, or NULL with codes and scales: its 8-bit rows.
  * dy has element type y_dtype.  dx must not overlap the inputs.  rows == 0 gives
- * zero dw and db.  The sums over rows have a fixed order.
+ * zero dw and db.  The sums over rows have a fixed order.  *d_status (may be
+ * NULL) receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up.
  */
 IFK_API int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const void* x, int64_t ld_x,
                                    int x_dtype, const int8_t* codes, int64_t ld_codes,
                                    const uint8_t* scales, int64_t ld_scales, const float* mean,
                                    const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n,
-                                   void* dx, int64_t ld_dx, float* dw, float* db, void* workspace,
-                                   size_t workspace_bytes, ifk_stream_t stream);
+                                   void* dx, int64_t ld_dx, float* dw, float* db, int* d_status,
+                                   void* workspace, size_t workspace_bytes, ifk_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -121,7 +121,7 @@ def test_layernorm_argument_errors_before_any_gpu_work():
     def bwd(dy=FAKE, ldy=64, yd=_lib.F32, x=FAKE, ldx=64, xd=_lib.F32, codes=None, scales=None, mean=FAKE, w=FAKE,
             wd=_lib.F32, dx=FAKE, lddx=64, dw=FAKE, ws=FAKE, wsb=need):
         return L.ifk_layernorm_backward(dy, ldy, yd, x, ldx, xd, codes, 64, scales, 2, mean, FAKE, w, wd, 4, 64, dx,
-                                        lddx, dw, None, ws, wsb, None)
+                                        lddx, dw, None, None, ws, wsb, None)
 
     assert bwd(dy=None) == _lib.ERR_ARG
     assert bwd(mean=None) == _lib.ERR_ARG

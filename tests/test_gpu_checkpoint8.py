@@ -218,13 +218,17 @@ def ln_tolerance(x, z, rstd, mean, n):
 
 LN_SIZES = [(1, 1, 0), (1, 2048, 0), (3, 2, 0), (5, 31, 0), (17, 64, 0), (33, 256, 8), (40, 257, 0), (9, 512, 1),
             (300, 768, 0), (12, 1000, 4), (50, 1024, 0), (21, 1537, 7), (11, 2056, 0), (6, 4096, 0), (3, 8191, 3),
-            (4, 8192, 0), (2, 16384, 0), (2, 20001, 0), (1300, 40, 0), (700, 1280, 0)]
+            (4, 8192, 0), (2, 16384, 0), (2, 20001, 0), (1300, 40, 0), (700, 1280, 0),
+            # rows enough to be walked through rings in shared memory
+            (4800, 96, 0), (2501, 1280, 0), (2600, 768, 8), (1300, 4096, 0), (310, 8192, 0), (605, 6000, 16),
+            (300, 16384, 0)]
 
 
 @pytest.mark.parametrize("xd,yd", [(F4, F4), (F4, BF), (BF, BF), (BF, F4)])
 @pytest.mark.parametrize("rows,n,pad", LN_SIZES)
 def test_layer_norm(rows, n, pad, xd, yd):
     x = buffer(rows, n, xd, pad, seed=n, spread=8.0) + (0.5 if pad == 0 else 0.0)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
     g = torch.Generator(device="cuda").manual_seed(rows)
     w = 1 + 0.1 * torch.randn(n, generator=g, device="cuda")
     b = 0.1 * torch.randn(n, generator=g, device="cuda")
@@ -244,7 +248,8 @@ def test_layer_norm(rows, n, pad, xd, yd):
             assert torch.equal(q.codes, saved.q8.codes) and torch.equal(q.scales, saved.q8.scales)
             z = (c8().dequantize_rows(q, F4).double() - M) * R
             tzq = ln_tolerance(x.double(), z, R, M, n)
-        dx, dw, db = c8().layer_norm_backward(dy, saved, w)
+        dx, dw, db = c8().layer_norm_backward(dy, saved, w, status=status)
+        assert status.item() == 0
         DX, DW, DB = ref.layer_norm_backward(dy, z, R, w)
         gw = (dy.double() * w.double()).abs()
         k = (min(n, 96) + 8) * U2
