@@ -48,11 +48,11 @@ __device__ __forceinline__ float team_sum(float v, int W, float* buf) {
 
 // 8-bit rows of x, written as ifk_q8_quantize writes them.
 template <int V>
-__device__ __forceinline__ void write_codes(const FwdArgs& a, int64_t row, int c, const float (&v)[V]) {
+__device__ __forceinline__ void write_codes(int8_t* codes, uint8_t* scales, int pitch, int c, const float (&v)[V]) {
   const uint32_t m = q8::group_max_bits<V>(v), s = q8::scale_byte(m);
-  if (c >= a.pitch) return;
-  q8::store_codes<V>(a.codes + row * a.ldc + c, v, m, s);
-  if ((c & (q8::GROUP - 1)) == 0) a.scales[row * a.lds + c / q8::GROUP] = (uint8_t)s;
+  if (c >= pitch) return;
+  q8::store_codes<V>(codes + c, v, m, s);
+  if ((c & (q8::GROUP - 1)) == 0) scales[c / q8::GROUP] = (uint8_t)s;
 }
 
 // The mean is taken twice: the second sum, over x less the first mean, carries what the
@@ -92,10 +92,17 @@ __device__ __forceinline__ void write_out(const FwdArgs& a, TY* y, int c, const 
   store_vec<V, PLAIN>(y, c, a.n, o);
 }
 
-template <typename TX, typename TY, int V, int NV, bool PLAIN>
-__global__ void __launch_bounds__(512, 2) forward_kernel(const FwdArgs a) {
+// WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
+template <int WARPS>
+constexpr int max_threads() { return WARPS == 0 ? 512 : WARPS == 1 ? 32 * ROWS_PER_BLOCK : 32 * WARPS; }
+// 64 registers a thread, 85 with 64 columns.
+template <int WARPS, int COLS>
+constexpr int min_blocks() { return (COLS > 32 ? 768 : 1024) / max_threads<WARPS>(); }
+
+template <typename TX, typename TY, int V, int NV, bool PLAIN, int WARPS>
+__global__ void __launch_bounds__(max_threads<WARPS>(), min_blocks<WARPS, V * NV>()) forward_kernel(const FwdArgs a) {
   __shared__ float buf[3][32];
-  const int W = a.W, lane = threadIdx.x & 31;
+  const int W = WARPS ? WARPS : a.W, lane = threadIdx.x & 31;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * ROWS_PER_BLOCK + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;  // whole warps of one-warp rows
   const int c0 = (W == 1 ? lane : (int)threadIdx.x) * V, step = 32 * W * V;
@@ -186,12 +193,14 @@ __global__ void __launch_bounds__(512, 2) forward_kernel(const FwdArgs a) {
     if (a.mean) a.mean[row] = t.m1 + t.c1;
     if (a.rstd) a.rstd[row] = t.rstd;
   }
+  int8_t* codes = a.codes + row * a.ldc;
+  uint8_t* scales = a.scales + row * a.lds;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = c0 + k * step;
     float v[V];
     unpack(r[k], v);
-    if (a.codes) write_codes<V>(a, row, c, v);
+    if (a.codes) write_codes<V>(codes, scales, a.pitch, c, v);
     if (c < a.n) write_out<TY, V, PLAIN>(a, y, c, v, t);
   }
 }
@@ -233,25 +242,30 @@ __global__ void __launch_bounds__(512) forward_long_kernel(const FwdArgs a) {
   for (int cw = (threadIdx.x & ~31) * V; cw < a.pitch; cw += step) {
     const int c = cw + (threadIdx.x & 31) * V;
     unpack(load_raw<TX, V>(x, c, a.n), v);
-    if (a.codes) write_codes<V>(a, row, c, v);
+    if (a.codes) write_codes<V>(a.codes + row * a.ldc, a.scales + row * a.lds, a.pitch, c, v);
     if (c < a.n) write_out<TY, V, false>(a, y, c, v, t);
   }
 }
 
 template <typename TX, typename TY, int V, int NV, bool PLAIN>
 void launch(FwdArgs& a, cudaStream_t s) {
+  const unsigned rows = (unsigned)a.rows;
   if (a.W == 1)
-    forward_kernel<TX, TY, V, NV, PLAIN>
+    forward_kernel<TX, TY, V, NV, PLAIN, 1>
         <<<(unsigned)cdiv(a.rows, ROWS_PER_BLOCK), 32 * ROWS_PER_BLOCK, 0, s>>>(a);
+  else if (PLAIN && a.W == 2)
+    forward_kernel<TX, TY, V, NV, PLAIN, PLAIN ? 2 : 0><<<rows, 32 * a.W, 0, s>>>(a);
+  else if (PLAIN && a.W == 4)
+    forward_kernel<TX, TY, V, NV, PLAIN, PLAIN ? 4 : 0><<<rows, 32 * a.W, 0, s>>>(a);
   else
-    forward_kernel<TX, TY, V, NV, PLAIN><<<(unsigned)a.rows, 32 * a.W, 0, s>>>(a);
+    forward_kernel<TX, TY, V, NV, PLAIN, 0><<<rows, 32 * a.W, 0, s>>>(a);
 }
 
-// Accesses a lane makes of a row: 32 columns' at most; fewer, by more warps a row, while the rows alone
+// Accesses a lane makes of a row: 32 columns' at most, 64 where both sides are bf16; fewer, by more warps a row, while the rows alone
 // do not give each SM eight warps.
 template <typename TX, typename TY, int V>
 int forward(FwdArgs& a, cudaStream_t s) {
-  constexpr int MAXV = 32 / V;
+  constexpr int MAXV = V == 8 ? 8 : 32 / V;
   const int acc = a.pitch / V;  // accesses of a row (with the padding of its last group)
   int W = (int)cdiv(acc, 32 * MAXV);
   if (W > 16) {
@@ -273,10 +287,10 @@ int forward(FwdArgs& a, cudaStream_t s) {
       launch<TX, TY, V, 1, true>(a, s);
     } else if (nv <= 2) {
       launch<TX, TY, V, 2, true>(a, s);
-    } else if (V == 8 ? nv <= 3 : nv <= 4) {
-      launch<TX, TY, V, V == 8 ? 3 : 4, true>(a, s);
-    } else if (V == 4 && nv <= 6) {
-      launch<TX, TY, V, V == 4 ? 6 : MAXV, true>(a, s);
+    } else if (nv <= 4) {
+      launch<TX, TY, V, 4, true>(a, s);
+    } else if (nv <= 6) {
+      launch<TX, TY, V, 6, true>(a, s);
     } else {
       launch<TX, TY, V, MAXV, true>(a, s);
     }

@@ -147,13 +147,14 @@ __global__ void __launch_bounds__(512, 1) backward_kernel(const BwdArgs a) {
 
 // Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
 // A wait that gives up marks the call and the block goes on (its result is not valid).
-template <typename TX, typename TY, int V, int COLS, bool Q8>
+// WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
+template <typename TX, typename TY, int V, int COLS, int WARPS, bool Q8>
 __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_kernel(const BwdArgs a) {
   constexpr int NV = COLS / V, H = V / 2;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 buf[2][16];
   __shared__ int failed;
-  const int W = a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
+  const int W = WARPS ? WARPS : a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
   const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
   const bool leader = lane == 0 && warp == team * W;
   const int dy_bytes = a.n * (int)sizeof(TY);
@@ -194,10 +195,8 @@ __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_ker
     rstd = a.rstd[row];
     if (Q8) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = c0 + k * step;
-        sc[k % (Q8 ? NV : 1)] = c < a.n ? a.scales[row * a.lds + c / q8::GROUP] : 0;
-      }
+      for (int k = 0; k < NV; ++k)
+        sc[k % (Q8 ? NV : 1)] = c0 + k * step < a.n ? a.scales[row * a.lds + (c0 + k * step) / q8::GROUP] : 0;
     }
   };
   if (first < a.rows) ahead(first);
@@ -361,7 +360,11 @@ __global__ void __launch_bounds__(256) backward_long_sums_kernel(const BwdArgs a
 
 // Persistent blocks: one an SM, fewer when the rows do not fill them (a block's partial sums are written
 // and read once).  The number of blocks depends on the sizes alone: it is the number of partial sums.
-int row_warps(int64_t n) { return n <= NARROW ? 1 : (int)cdiv(n, 32 * 16); }
+int row_warps(int64_t n) {
+  if (n <= NARROW) return 1;
+  const int w = (int)cdiv(n, 32 * 16);
+  return w <= 4 ? w : w <= 6 ? 6 : w <= 8 ? 8 : w;
+}
 int64_t parts_of(int64_t rows, int64_t n) {
   if (row_warps(n) > MAX_W) return std::min<int64_t>(cdiv(rows, 64), 32);
   const int teams = n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / row_warps(n));
@@ -394,10 +397,10 @@ int launch(K kernel, int* done_dev, unsigned blocks, unsigned threads, size_t sm
   return IFK_OK;
 }
 
-template <typename TX, typename TY, int V, int COLS, bool Q8>
+template <typename TX, typename TY, int V, int COLS, int WARPS, bool Q8>
 int launch_ring(const BwdArgs& a, unsigned blocks, size_t row, cudaStream_t s) {
   static thread_local int done_dev = -1;
-  return launch(backward_ring_kernel<TX, TY, V, COLS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
+  return launch(backward_ring_kernel<TX, TY, V, COLS, WARPS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
                 std::max<size_t>(a.teams * a.depth * (row + 8), sums_bytes(a)), a, s);
 }
 
@@ -415,9 +418,16 @@ int backward(BwdArgs& a, cudaStream_t s) {
   a.teams = a.n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / a.W);
   if constexpr (V > 1) {
     size_t row;
-    if (ring_ok<TX, TY, V, Q8>(a, &row))
-      return a.n <= NARROW ? launch_ring<TX, TY, V, 32, Q8>(a, parts, row, s)
-                           : launch_ring<TX, TY, V, 16, Q8>(a, parts, row, s);
+    if (ring_ok<TX, TY, V, Q8>(a, &row)) {
+      switch (a.W) {
+        case 1: return launch_ring<TX, TY, V, 32, 1, Q8>(a, parts, row, s);
+        case 3: return launch_ring<TX, TY, V, 16, 3, Q8>(a, parts, row, s);
+        case 4: return launch_ring<TX, TY, V, 16, 4, Q8>(a, parts, row, s);
+        case 6: return launch_ring<TX, TY, V, 16, 6, Q8>(a, parts, row, s);
+        case 8: return launch_ring<TX, TY, V, 16, 8, Q8>(a, parts, row, s);
+        default: return launch_ring<TX, TY, V, 16, 0, Q8>(a, parts, row, s);
+      }
+    }
   }
   a.W = (int)cdiv(a.n, 32 * 16);
   a.teams = std::max(1, 16 / a.W);
