@@ -6,7 +6,8 @@
 // db in registers, and a ring of rows in shared memory a team, that bulk copies keep
 // filled.  At the end the block adds its teams' sums in shared memory and writes one row
 // of partial sums; a second kernel adds the blocks'.  The order of every sum is fixed by
-// the sizes.  fp32 arithmetic goes two to an instruction (F2): the instructions, not the
+// the sizes.  The weight is in shared memory, too: beside the ring there is little L1 left, and
+// from L2 it took a third of a row's time.  fp32 arithmetic goes two to an instruction (F2): the instructions, not the
 // memory, bound a row of 768 columns in 8 bits otherwise.
 #include <algorithm>
 #include <cstring>
@@ -18,6 +19,9 @@
 namespace ifk {
 
 namespace {
+
+// Bytes of the weight's copy in shared memory (whole blocks of 256 columns).
+__host__ __device__ inline size_t weight_bytes(int n) { return (size_t)cdiv(n, 256) * 256 * sizeof(float); }
 
 struct BwdArgs {
   const void* dy;
@@ -145,6 +149,13 @@ __global__ void __launch_bounds__(512, 1) backward_kernel(const BwdArgs a) {
   if (a.part) write_sums<V, NV>(a, team, c0, step, sw, sb, sums);
 }
 
+// Where a row's column c stands in the weight's copy in shared memory: the halves of 8 columns a lane
+// apart, so that a warp's 16-byte reads are contiguous.
+template <int V>
+__device__ __forceinline__ int weight_at(int c) {
+  return V == 8 ? (c & ~255) + (c & 4) * 32 + ((c >> 1) & 124) + (c & 3) : c;
+}
+
 // Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
 // A wait that gives up marks the call and the block goes on (its result is not valid).
 // WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
@@ -159,9 +170,11 @@ __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_ker
   const bool leader = lane == 0 && warp == team * W;
   const int dy_bytes = a.n * (int)sizeof(TY);
   const int x_bytes = Q8 ? (int)q8::pitch(a.n) : a.n * (int)sizeof(TX), bytes = dy_bytes + x_bytes;
-  uint8_t* ring = smem + (size_t)team * a.depth * bytes;
+  float* weight = reinterpret_cast<float*>(smem);
+  uint8_t* rings = smem + weight_bytes(a.n);
+  uint8_t* ring = rings + (size_t)team * a.depth * bytes;
   const uint32_t data = (uint32_t)__cvta_generic_to_shared(ring);
-  const uint32_t full = (uint32_t)__cvta_generic_to_shared(smem + (size_t)a.teams * a.depth * bytes) +
+  const uint32_t full = (uint32_t)__cvta_generic_to_shared(rings + (size_t)a.teams * a.depth * bytes) +
                         (uint32_t)(team * a.depth * 8);
   const int64_t stride = (int64_t)gridDim.x * a.teams, first = (int64_t)blockIdx.x * a.teams + team;
   if (threadIdx.x == 0) failed = 0;
@@ -169,6 +182,11 @@ __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_ker
     for (int i = 0; i < a.depth; ++i)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
+    float w = 1.f;
+    if (a.w) w = a.w_bf16 ? __bfloat162float(((const __nv_bfloat16*)a.w)[c]) : ((const float*)a.w)[c];
+    weight[weight_at<V>(c)] = w;
   }
   __syncthreads();
   auto fetch = [&](int64_t row, int slot) {
@@ -181,7 +199,6 @@ __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_ker
   if (leader)
     for (int i = 0; i < a.depth && first + i * stride < a.rows; ++i) fetch(first + i * stride, i);
   const float inv_n = 1.f / (float)a.n;
-  const bool w_f32 = a.w && !a.w_bf16;
   F2 sw[NV][H], sb[NV][H];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -225,9 +242,12 @@ __global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_ker
         pairs(v, z[k]);
       }
       F2 w[H];
-      if (w_f32) load_f32<V>((const float*)a.w, c, v);
-      else load_param<V>(a.w, a.w_bf16, 1.f, c, a.n, v);
-      pairs(v, w);
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(weight + weight_at<V>(c + j));
+        w[j / 2] = f2(q.x, q.y);
+        w[j / 2 + 1] = f2(q.z, q.w);
+      }
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         z[k][i] = mul(add(z[k][i], nmu), rs2);
@@ -378,7 +398,7 @@ template <typename TX, typename TY, int V, bool Q8>
 bool ring_ok(BwdArgs& a, size_t* row) {
   const size_t dy = (size_t)a.n * sizeof(TY), x = Q8 ? (size_t)q8::pitch(a.n) : (size_t)a.n * sizeof(TX);
   *row = dy + x;
-  a.depth = (int)std::min<size_t>(8, RING_BYTES / (a.teams * *row));
+  a.depth = (int)std::min<size_t>(8, (RING_BYTES - weight_bytes(a.n)) / (a.teams * *row));
   return V > 1 && a.n % V == 0 && a.depth >= 2 && dy % 16 == 0 && x % 16 == 0 &&
          rows_allow<uint8_t>(a.dy, a.lddy * (int64_t)sizeof(TY), 16) &&
          (Q8 || rows_allow<uint8_t>(a.x, a.ldx * (int64_t)sizeof(TX), 16));
@@ -401,7 +421,7 @@ template <typename TX, typename TY, int V, int COLS, int WARPS, bool Q8>
 int launch_ring(const BwdArgs& a, unsigned blocks, size_t row, cudaStream_t s) {
   static thread_local int done_dev = -1;
   return launch(backward_ring_kernel<TX, TY, V, COLS, WARPS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
-                std::max<size_t>(a.teams * a.depth * (row + 8), sums_bytes(a)), a, s);
+                std::max<size_t>(weight_bytes(a.n) + a.teams * a.depth * (row + 8), sums_bytes(a)), a, s);
 }
 
 template <typename TX, typename TY, int V, bool Q8>
