@@ -271,9 +271,9 @@ def _affine(n: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]
     t = weight if weight is not None else bias
     if t is None:
         return _lib.F32
-    for p, name in ((weight, "weight"), (bias, "bias")):
-        if p is not None and (p.shape != (n,) or not p.is_contiguous()):
-            raise ValueError(f"{name} must hold {n} contiguous values, got shape {tuple(p.shape)}")
+    for p in (weight, bias):
+        if p is not None and (p.dim() != 1 or p.numel() != n or not p.is_contiguous()):
+            raise ValueError(f"weight and bias must hold {n} contiguous values, got shape {tuple(p.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight and bias share a dtype, got {weight.dtype} and {bias.dtype}")
     return _code(t.dtype)

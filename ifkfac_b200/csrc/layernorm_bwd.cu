@@ -40,11 +40,10 @@ struct BwdArgs {
   int* status;
 };
 
-// A lane holds 32 columns of a row of up to 1024 columns (one warp, no barrier), else 16.
-constexpr int NARROW = 1024;
-constexpr int MAX_W = 16;  // warps a row: up to 32 * 16 * 16 = 8192 columns
-template <int COLS>
-constexpr int block_warps() { return COLS == 32 ? 12 : 16; }  // 168 or 128 registers a thread
+constexpr int COLS = 16;         // columns a lane holds: 32 left too few warps for the registers (120 against 80 us
+                                 // for 65536 rows of 768 columns in 8 bits)
+constexpr int MAX_W = 16;        // warps a row: up to 32 * 16 * 16 = 8192 columns
+constexpr int BLOCK_WARPS = 16;  // 128 registers a thread
 
 // The block's sums over its rows: the teams' go to shared memory (2 n floats a team) and are added in order.
 template <int V, int NV>
@@ -88,9 +87,9 @@ __device__ __forceinline__ void row_part(const BwdArgs& a, int64_t row, int c, f
 
 // Rows straight from memory: any alignment and width.
 template <typename TX, typename TY, int V, bool Q8>
-__global__ void __launch_bounds__(512, 1) backward_kernel(const BwdArgs a) {
-  constexpr int NV = 16 / V;
-  __shared__ float2 buf[2][16];
+__global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_kernel(const BwdArgs a) {
+  constexpr int NV = COLS / V;
+  __shared__ float2 buf[2][BLOCK_WARPS];
   extern __shared__ float sums[];
   const int W = a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
   const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
@@ -159,11 +158,11 @@ __device__ __forceinline__ int weight_at(int c) {
 // Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
 // A wait that gives up marks the call and the block goes on (its result is not valid).
 // WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
-template <typename TX, typename TY, int V, int COLS, int WARPS, bool Q8>
-__global__ void __launch_bounds__(32 * block_warps<COLS>(), 1) backward_ring_kernel(const BwdArgs a) {
+template <typename TX, typename TY, int V, int WARPS, bool Q8>
+__global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(const BwdArgs a) {
   constexpr int NV = COLS / V, H = V / 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 buf[2][16];
+  __shared__ float2 buf[2][BLOCK_WARPS];
   __shared__ int failed;
   const int W = WARPS ? WARPS : a.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / W;
   const int c0 = ((warp - team * W) * 32 + lane) * V, step = 32 * W * V;
@@ -381,14 +380,13 @@ __global__ void __launch_bounds__(256) backward_long_sums_kernel(const BwdArgs a
 // Persistent blocks: one an SM, fewer when the rows do not fill them (a block's partial sums are written
 // and read once).  The number of blocks depends on the sizes alone: it is the number of partial sums.
 int row_warps(int64_t n) {
-  if (n <= NARROW) return 1;
-  const int w = (int)cdiv(n, 32 * 16);
-  return w <= 4 ? w : w <= 6 ? 6 : w <= 8 ? 8 : w;
+  const int w = (int)cdiv(n, 32 * COLS);
+  return w == 5 ? 6 : w == 7 ? 8 : w;  // the counts that have a kernel of their own
 }
+int block_teams(int64_t n) { return std::max(1, BLOCK_WARPS / row_warps(n)); }
 int64_t parts_of(int64_t rows, int64_t n) {
   if (row_warps(n) > MAX_W) return std::min<int64_t>(cdiv(rows, 64), 32);
-  const int teams = n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / row_warps(n));
-  return std::min<int64_t>(cdiv(rows, teams), 148);
+  return std::min<int64_t>(cdiv(rows, block_teams(n)), 148);
 }
 
 constexpr size_t RING_BYTES = 200 * 1024;
@@ -417,10 +415,10 @@ int launch(K kernel, int* done_dev, unsigned blocks, unsigned threads, size_t sm
   return IFK_OK;
 }
 
-template <typename TX, typename TY, int V, int COLS, int WARPS, bool Q8>
+template <typename TX, typename TY, int V, int WARPS, bool Q8>
 int launch_ring(const BwdArgs& a, unsigned blocks, size_t row, cudaStream_t s) {
   static thread_local int done_dev = -1;
-  return launch(backward_ring_kernel<TX, TY, V, COLS, WARPS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
+  return launch(backward_ring_kernel<TX, TY, V, WARPS, Q8>, &done_dev, blocks, 32 * a.W * a.teams,
                 std::max<size_t>(weight_bytes(a.n) + a.teams * a.depth * (row + 8), sums_bytes(a)), a, s);
 }
 
@@ -435,22 +433,21 @@ int backward(BwdArgs& a, cudaStream_t s) {
     IFK_CUDA_TRY(cudaGetLastError());
     return IFK_OK;
   }
-  a.teams = a.n <= NARROW ? block_warps<32>() : std::max(1, block_warps<16>() / a.W);
+  a.teams = block_teams(a.n);
   if constexpr (V > 1) {
     size_t row;
     if (ring_ok<TX, TY, V, Q8>(a, &row)) {
       switch (a.W) {
-        case 1: return launch_ring<TX, TY, V, 32, 1, Q8>(a, parts, row, s);
-        case 3: return launch_ring<TX, TY, V, 16, 3, Q8>(a, parts, row, s);
-        case 4: return launch_ring<TX, TY, V, 16, 4, Q8>(a, parts, row, s);
-        case 6: return launch_ring<TX, TY, V, 16, 6, Q8>(a, parts, row, s);
-        case 8: return launch_ring<TX, TY, V, 16, 8, Q8>(a, parts, row, s);
-        default: return launch_ring<TX, TY, V, 16, 0, Q8>(a, parts, row, s);
+        case 1: return launch_ring<TX, TY, V, 1, Q8>(a, parts, row, s);
+        case 2: return launch_ring<TX, TY, V, 2, Q8>(a, parts, row, s);
+        case 3: return launch_ring<TX, TY, V, 3, Q8>(a, parts, row, s);
+        case 4: return launch_ring<TX, TY, V, 4, Q8>(a, parts, row, s);
+        case 6: return launch_ring<TX, TY, V, 6, Q8>(a, parts, row, s);
+        case 8: return launch_ring<TX, TY, V, 8, Q8>(a, parts, row, s);
+        default: return launch_ring<TX, TY, V, 0, Q8>(a, parts, row, s);
       }
     }
   }
-  a.W = (int)cdiv(a.n, 32 * 16);
-  a.teams = std::max(1, 16 / a.W);
   static thread_local int done_dev = -1;
   return launch(backward_kernel<TX, TY, V, Q8>, &done_dev, parts, 32 * a.W * a.teams, sums_bytes(a), a, s);
 }
