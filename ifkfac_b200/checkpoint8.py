@@ -45,30 +45,29 @@ def _code(dtype: torch.dtype) -> int:
         raise TypeError(f"ifkfac_b200 supports float32 and bfloat16 tensors, got {dtype}") from None
 
 
-def _need_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
-    """The one CUDA device of the tensors (None entries are skipped)."""
-    dev = None
+def _need_cuda(*ts: Optional[torch.Tensor]) -> int:
+    """The index of the one CUDA device of the tensors (None entries are skipped)."""
+    dev = -2
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("ifkfac_b200 operates on CUDA tensors only (no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}: one call works on one device")
+        if t is not None:
+            i = t.get_device()
+            if i != dev:
+                if i < 0:
+                    raise ValueError("ifkfac_b200 operates on CUDA tensors only (no CPU path)")
+                if dev >= 0:
+                    raise ValueError(f"tensors on devices {dev} and {i}: one call works on one device")
+                dev = i
     return dev
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
-    """A library call on the current stream of ``dev``, which is made current for it."""
+def _call(name: str, dev: int, *args) -> None:
+    """A library call on the current stream of device ``dev``, which is made current for it."""
     fn = getattr(_lib.lib(), name)
-    i = dev.index
-    if torch._C._cuda_getDevice() == i:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(i):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise IFKError(rc, name)
 
@@ -96,10 +95,10 @@ class Q8Rows:
     multiple of 32), ``scales`` (rows x pitch / 32 uint8).  Slices along the rows are
     views of the same storage.
 
-    Rows made here keep codes and scales in one buffer, ``data`` (the codes of all
-    rows, then the scales)."""
+    Rows made here keep codes and scales in one uint8 buffer, ``data`` (from byte
+    ``start`` on the codes of all rows, then the scales)."""
 
-    __slots__ = ("rows", "cols", "data", "_codes", "_scales")
+    __slots__ = ("rows", "cols", "data", "start", "_codes", "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
         cols = int(cols)
@@ -113,32 +112,41 @@ class Q8Rows:
         (ldc, uc), (lds, us) = codes.stride(), scales.stride()
         if rows > 1 and (ldc < pitch or lds < pitch // _G) or uc != 1 or (us != 1 and pitch > _G):
             raise ValueError("codes and scales must be row-major")
-        self.rows, self.cols, self.data, self._codes, self._scales = rows, cols, None, codes, scales
+        self.rows, self.cols, self.data, self.start, self._codes, self._scales = rows, cols, None, 0, codes, scales
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Q8Rows":
-        pitch = -(-cols // _G) * _G
-        return cls.of(torch.empty(rows * (pitch + pitch // _G), dtype=torch.uint8, device=device), rows, cols)
+        return cls.of(torch.empty(cls.size(rows, cols), dtype=torch.uint8, device=device), rows, cols)
+
+    @staticmethod
+    def size(rows: int, cols: int) -> int:
+        """Bytes of the rows in one buffer."""
+        groups = -(-cols // _G)
+        return rows * groups * (_G + 1)
 
     @classmethod
-    def of(cls, data: torch.Tensor, rows: int, cols: int) -> "Q8Rows":
-        """The rows in a buffer laid out as ``data``."""
+    def of(cls, data: torch.Tensor, rows: int, cols: int, start: int = 0) -> "Q8Rows":
+        """The rows in a buffer laid out as ``data`` (``start`` a multiple of 16)."""
         q = cls.__new__(cls)
-        q.rows, q.cols, q.data, q._codes, q._scales = rows, cols, data, None, None
+        q.rows, q.cols, q.data, q.start, q._codes, q._scales = rows, cols, data, start, None, None
         return q
+
+    def _split(self) -> None:
+        groups = -(-self.cols // _G)
+        mid = self.start + self.rows * groups * _G
+        self._codes = self.data[self.start: mid].view(torch.int8).view(self.rows, groups * _G)
+        self._scales = self.data[mid: mid + self.rows * groups].view(self.rows, groups)
 
     @property
     def codes(self) -> torch.Tensor:
         if self._codes is None:
-            pitch = -(-self.cols // _G) * _G
-            self._codes = self.data[: self.rows * pitch].view(torch.int8).view(self.rows, pitch)
+            self._split()
         return self._codes
 
     @property
     def scales(self) -> torch.Tensor:
         if self._scales is None:
-            pitch = -(-self.cols // _G) * _G
-            self._scales = self.data[self.rows * pitch:].view(self.rows, pitch // _G)
+            self._split()
         return self._scales
 
     @property
@@ -147,8 +155,7 @@ class Q8Rows:
 
     @property
     def nbytes(self) -> int:
-        pitch = -(-self.cols // _G) * _G
-        return self.rows * (pitch + pitch // _G)
+        return self.size(self.rows, self.cols)
 
     def tensors(self) -> Tuple[torch.Tensor, ...]:
         """The tensors that hold the rows."""
@@ -156,12 +163,13 @@ class Q8Rows:
 
     def args(self) -> Tuple[int, int, int, int]:
         """(codes, ld, scales, ld) of a library call."""
-        pitch = -(-self.cols // _G) * _G
+        groups = -(-self.cols // _G)
+        pitch = groups * _G
         if self.data is not None:
-            p = self.data.data_ptr()
-            return p, pitch, p + self.rows * pitch, pitch // _G
+            p = self.data.data_ptr() + self.start
+            return p, pitch, p + self.rows * pitch, groups
         c, s = self._codes, self._scales
-        return c.data_ptr(), max(c.stride(0), pitch), s.data_ptr(), max(s.stride(0), pitch // _G)
+        return c.data_ptr(), max(c.stride(0), pitch), s.data_ptr(), max(s.stride(0), groups)
 
     def __getitem__(self, rows: slice) -> "Q8Rows":
         if not isinstance(rows, slice) or rows.step not in (None, 1):
@@ -172,10 +180,10 @@ class Q8Rows:
         return f"Q8Rows({self.rows} x {self.cols}, {self.device})"
 
 
-def _index(index: torch.Tensor, dev: torch.device) -> torch.Tensor:
+def _index(index: torch.Tensor, dev: int) -> torch.Tensor:
     if index.dim() != 1 or index.dtype not in (torch.int64, torch.int32):
         raise ValueError("a row index is a 1-D integer tensor")
-    return index.to(device=dev, dtype=torch.int64).contiguous()
+    return index.to(device=torch.device("cuda", dev), dtype=torch.int64).contiguous()
 
 
 def quantize_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None,
@@ -248,23 +256,37 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
 
 
 class LayerNormSaved:
-    """What layer norm's backward pass needs of its forward pass: the statistics (``stats``,
-    2 x rows fp32: means, then reciprocal deviations) and the input rows, as they were
-    (``x``) or in 8 bits (``q8``)."""
+    """What layer norm's backward pass needs of its forward pass: the input rows, as they
+    were (``x``) or in 8 bits (``q8``), and the statistics: ``data`` begins with the
+    rows' means and then their reciprocal deviations (fp32)."""
 
-    __slots__ = ("x", "q8", "stats", "x_dtype", "rows", "cols")
+    __slots__ = ("x", "q8", "data", "x_dtype", "rows", "cols")
 
-    def __init__(self, x: Optional[torch.Tensor], q8: Optional[Q8Rows], stats: torch.Tensor, x_dtype: torch.dtype,
+    def __init__(self, x: Optional[torch.Tensor], q8: Optional[Q8Rows], data: torch.Tensor, x_dtype: torch.dtype,
                  rows: int, cols: int):
-        self.x, self.q8, self.stats, self.x_dtype, self.rows, self.cols = x, q8, stats, x_dtype, rows, cols
+        self.x, self.q8, self.data, self.x_dtype, self.rows, self.cols = x, q8, data, x_dtype, rows, cols
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, x_dtype: torch.dtype, device, x: Optional[torch.Tensor]) -> "LayerNormSaved":
+        """Room for the statistics of ``x`` and, where the rows themselves are not kept
+        (``x`` None), for them in 8 bits."""
+        start = -(-8 * rows // 16) * 16
+        nbytes = start if x is not None else start + Q8Rows.size(rows, cols)
+        return cls.of(torch.empty(nbytes, dtype=torch.uint8, device=device), rows, cols, x_dtype, x)
+
+    @classmethod
+    def of(cls, data: torch.Tensor, rows: int, cols: int, x_dtype: torch.dtype,
+           x: Optional[torch.Tensor] = None) -> "LayerNormSaved":
+        start = -(-8 * rows // 16) * 16
+        return cls(x, None if x is not None else Q8Rows.of(data, rows, cols, start), data, x_dtype, rows, cols)
 
     @property
     def mean(self) -> torch.Tensor:
-        return self.stats[0]
+        return self.data[: 4 * self.rows].view(torch.float32)
 
     @property
     def rstd(self) -> torch.Tensor:
-        return self.stats[1]
+        return self.data[4 * self.rows: 8 * self.rows].view(torch.float32)
 
 
 def _affine(n: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
@@ -300,14 +322,11 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     saved = mean = rstd = None
     q = _NO_ROWS
     if save:
-        stats = torch.empty(2, rows, dtype=torch.float32, device=dev)
-        mean = stats.data_ptr()
+        saved = LayerNormSaved.empty(rows, n, x.dtype, dev, None if checkpoint else x)
+        mean = saved.data.data_ptr()
         rstd = mean + 4 * rows
-        q8 = None
         if checkpoint:
-            q8 = Q8Rows.empty(rows, n, dev)
-            q = q8.args()
-        saved = LayerNormSaved(None if checkpoint else x, q8, stats, x.dtype, rows, n)
+            q = saved.q8.args()
     _call("ifk_layernorm", dev, x.data_ptr(), ld, dt, _ptr(weight), _ptr(bias), wdt, rows, n, float(eps),
           y.data_ptr(), n, ydt, mean, rstd, *q)
     return y, saved
@@ -319,7 +338,7 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
     """(dx, dw, db) of :func:`layer_norm_forward`: dx in the input's dtype, dw and db
     fp32 (None without ``weight_grads``).  ``status`` (a device int32, optional)
     receives IFK_ERR_TIMEOUT if a wait on the device gave up."""
-    dev = _need_cuda(dy, saved.stats, weight, status)
+    dev = _need_cuda(dy, saved.data, weight, status)
     dy, rows, n, ld = _rows2d(dy, "dy")
     dt, xdt = _code(dy.dtype), _code(saved.x_dtype)
     if rows != saved.rows or n != saved.cols:
@@ -337,7 +356,7 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
         db = torch.empty(n, dtype=torch.float32, device=dev)
         nbytes = _lib.lib().ifk_layernorm_backward_workspace(rows, n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    mean = saved.stats.data_ptr()
+    mean = saved.data.data_ptr()
     _call("ifk_layernorm_backward", dev, dy.data_ptr(), ld, dt, x, ldx, xdt, *q, mean, mean + 4 * rows, _ptr(weight),
           wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(status), _ptr(ws), nbytes)
     return dx, dw, db
@@ -420,7 +439,7 @@ class _LayerNormQ8(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, dtype, save):
         y, s = layer_norm_forward(x.reshape(-1, x.shape[-1]), weight, bias, eps, dtype, save=save, checkpoint=True)
         if s is not None:
-            ctx.save_for_backward(s.stats, s.q8.data, *(() if weight is None else (weight,)))
+            ctx.save_for_backward(s.data, *(() if weight is None else (weight,)))
         ctx.x_dtype, ctx.x_shape = x.dtype, x.shape
         ctx.b_dtype = None if bias is None else bias.dtype
         return y.reshape(x.shape)
@@ -428,9 +447,9 @@ class _LayerNormQ8(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        stats, data, *w = ctx.saved_tensors
-        rows, n = stats.shape[1], ctx.x_shape[-1]
-        saved = LayerNormSaved(None, Q8Rows.of(data, rows, n), stats, ctx.x_dtype, rows, n)
+        data, *w = ctx.saved_tensors
+        n = ctx.x_shape[-1]
+        saved = LayerNormSaved.of(data, ctx.x_shape.numel() // n, n, ctx.x_dtype)
         weight = w[0] if w else None
         dx, dw, db = layer_norm_backward(dy.reshape(-1, n), saved, weight,
                                          weight_grads=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
