@@ -31,7 +31,9 @@ __device__ __forceinline__ int64_t source_row(int64_t i, const int64_t* ridx, in
 struct Units {
   int upr, rpb;
   uint32_t magic;  // ceil(2^32 / upr): u / upr is the high word of u magic, as u upr < 2^32 where rpb > 1
-  __device__ __forceinline__ uint32_t row(uint32_t u) const { return rpb == 1 ? 0u : __umulhi(u, magic); }
+  __device__ __forceinline__ uint32_t row(uint32_t u) const {
+    return rpb == 1 ? 0u : upr == 1 ? u : __umulhi(u, magic);  // 2^32 itself is no magic
+  }
 };
 
 // upr is a multiple of 32 / V: a group never spans two rows, and the lanes of a group are

@@ -33,7 +33,8 @@ def buffer(rows, n, dtype, pad=0, seed=0, spread=100.0, scale=1.0):
 
 @pytest.mark.parametrize("dtype", [BF, F4])
 @pytest.mark.parametrize("rows,n,pad", [(1, 1, 0), (1, 768, 0), (3, 31, 0), (5, 32, 0), (7, 33, 0), (300, 1025, 3),
-                                        (2, 70001, 0), (1000, 64, 8), (129, 257, 7)])
+                                        (2, 70001, 0), (1000, 64, 8), (129, 257, 7), (3000, 1, 0), (700, 3, 1),
+                                        (2500, 4, 4), (900, 8, 0), (600, 9, 7), (5000, 17, 0)])
 def test_quantize_matches_the_format_bit_for_bit(rows, n, pad, dtype):
     x = buffer(rows, n, dtype, pad, seed=n)
     if rows > 2:
