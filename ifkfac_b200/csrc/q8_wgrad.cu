@@ -521,16 +521,23 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
 
 // What is left when the tiles are summed.  The first `joins` blocks add a cut tile's shares, in the
 // order of the rows, 16 output columns a block: a thread has four 16-byte reads of a share in
-// flight.  The others add the parts of db, 32 columns a block.
+// flight.  The others add the parts of db, 32 columns a block, or, without parts, delta's few rows.
 constexpr int JOIN_COLS = 16;
-__global__ void __launch_bounds__(256) finish_kernel(const Args a, int joins, const float* sums, int parts, float* db) {
+constexpr int FEW_ROWS = 64;  // up to here a pass over delta of its own would cost more than these reads
+__global__ void __launch_bounds__(256)
+finish_kernel(const Args a, int joins, const float* sums, int parts, const __nv_bfloat16* delta, int64_t ldd,
+              float* db) {
   if ((int)blockIdx.x >= joins) {
     __shared__ float sh[8][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = (int64_t)(blockIdx.x - joins) * 32 + tx;
     float v = 0.f;
-    if (c < a.n_out)
-      for (int p = ty; p < parts; p += 8) v += sums[(int64_t)p * a.n_out + c];
+    if (c < a.n_out) {
+      if (delta)
+        for (int64_t r = ty; r < a.rows; r += 8) v += __bfloat162float(delta[r * ldd + c]);
+      else
+        for (int p = ty; p < parts; p += 8) v += sums[(int64_t)p * a.n_out + c];
+    }
     sh[ty][tx] = v;
     __syncthreads();
     if (ty == 0 && c < a.n_out) {
@@ -753,8 +760,8 @@ bool codes_map(CUtensorMap* m, const int8_t* c, int64_t ld, int64_t rows, int64_
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const float* sums, int parts, float* db,
-           cudaStream_t s) {
+int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const float* sums, int parts,
+           const __nv_bfloat16* delta, int64_t ldd, float* db, cudaStream_t s) {
   static thread_local int done_dev = -1;
   int dev = 0;
   IFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -776,7 +783,7 @@ int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const fl
   IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel, dm, cm, a));
   const int64_t joins = a.p.total && a.p.Gs > 1 ? a.p.total / a.p.Kt * (TN / JOIN_COLS) : 0;
   const int64_t blocks = joins + (db ? cdiv(a.n_out, 32) : 0);
-  if (blocks) finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(a, (int)joins, sums, parts, db);
+  if (blocks) finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(a, (int)joins, sums, parts, delta, ldd, db);
   IFK_CUDA_TRY(cudaGetLastError());
   return IFK_OK;
 }
@@ -813,7 +820,7 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
     IFK_CUDA_TRY(cudaGetLastError());
     src = terms;
     ld = l.ldo;
-  } else if (db) {
+  } else if (db && rows > FEW_ROWS) {
     delta_pass<TD, false>(delta, ldd, rows, n_out, parts, sums, nullptr, 0, s);
     IFK_CUDA_TRY(cudaGetLastError());
   }
@@ -821,7 +828,8 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.whole = n_out % 64 == 0;
   if (!delta_map(&dm, src, ld, rows, n_out, l.terms, a.whole) || !codes_map(&cm, codes, ldc, rows, n_in))
     return IFK_ERR_SHAPE;
-  return launch(dm, cm, a, sums, parts, db, s);
+  const bool few = !l.copy && rows <= FEW_ROWS;  // delta is bf16 then
+  return launch(dm, cm, a, sums, parts, few ? (const __nv_bfloat16*)(const void*)delta : nullptr, ldd, db, s);
 }
 
 }  // namespace

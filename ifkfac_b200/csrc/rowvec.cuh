@@ -11,6 +11,7 @@ template <typename T, int V>
 struct Raw;  // V elements as they are in memory
 template <> struct Raw<float, 4> { float4 r; };
 template <> struct Raw<float, 1> { float r; };
+template <> struct Raw<__nv_bfloat16, 16> { uint4 r, q; };
 template <> struct Raw<__nv_bfloat16, 8> { uint4 r; };
 template <> struct Raw<__nv_bfloat16, 4> { uint2 r; };
 template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 r; };
@@ -74,6 +75,16 @@ __device__ __forceinline__ void unpack(const Raw<__nv_bfloat16, 1>& q, float (&v
 __device__ __forceinline__ void unpack(const Raw<__nv_bfloat16, 4>& q, float (&v)[4]) {
   bf16x2(q.r.x, v[0], v[1]);
   bf16x2(q.r.y, v[2], v[3]);
+}
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16, 16>& q, float (&v)[16]) {
+  bf16x2(q.r.x, v[0], v[1]);
+  bf16x2(q.r.y, v[2], v[3]);
+  bf16x2(q.r.z, v[4], v[5]);
+  bf16x2(q.r.w, v[6], v[7]);
+  bf16x2(q.q.x, v[8], v[9]);
+  bf16x2(q.q.y, v[10], v[11]);
+  bf16x2(q.q.z, v[12], v[13]);
+  bf16x2(q.q.w, v[14], v[15]);
 }
 __device__ __forceinline__ void unpack(const Raw<__nv_bfloat16, 8>& q, float (&v)[8]) {
   bf16x2(q.r.x, v[0], v[1]);
@@ -221,7 +232,9 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&x)[V], uint
     w[j] = V == 1 ? e[0]
                   : __byte_perm(__byte_perm(e[(4 * j) % V], e[(4 * j + 1) % V], 0x0040),
                                 __byte_perm(e[(4 * j + 2) % V], e[(4 * j + 3) % V], 0x0040), 0x5410);
-  if (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[(V + 3) / 4 - 1]);
+  constexpr int N = (V + 3) / 4;
+  if (V == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1 % N], w[2 % N], w[3 % N]);
+  else if (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1 % N]);
   else if (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
   else *p = (int8_t)w[0];
 }
