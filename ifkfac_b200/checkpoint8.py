@@ -90,6 +90,14 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _status(t: Optional[torch.Tensor]):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() != 1:
+        raise TypeError(f"status is one int32 on the device, got {t.numel()} of {t.dtype}")
+    return t.data_ptr()
+
+
 class Q8Rows:
     """Rows in 8 bits: ``codes`` (rows x pitch int8, pitch = ``cols`` rounded up to a
     multiple of 32), ``scales`` (rows x pitch / 32 uint8).  Slices along the rows are
@@ -201,7 +209,7 @@ def quantize_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None,
         index = _index(index, dev)
         rows = index.numel()
     q = Q8Rows.empty(rows, cols, dev)
-    _call("ifk_q8_quantize", dev, x.data_ptr(), ld, dt, _ptr(index), src, rows, cols, *q.args(), _ptr(status))
+    _call("ifk_q8_quantize", dev, x.data_ptr(), ld, dt, _ptr(index), src, rows, cols, *q.args(), _status(status))
     return q
 
 
@@ -216,7 +224,7 @@ def dequantize_rows(q: Q8Rows, dtype: torch.dtype = torch.bfloat16, index: Optio
         rows = index.numel()
     out = torch.empty(rows, q.cols, dtype=dtype, device=dev)
     _call("ifk_q8_dequantize", dev, *q.args(), _ptr(index), q.rows, rows, q.cols, out.data_ptr(), q.cols, dt,
-          _ptr(status))
+          _status(status))
     return out
 
 
@@ -251,7 +259,7 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
     nbytes = _lib.lib().ifk_q8_wgrad_workspace(rows, n_out, n_in, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call("ifk_q8_wgrad", dev, delta.data_ptr(), ld, dt, *q.args(), rows, n_out, n_in, out.data_ptr(), ld_out,
-          _ptr(out_bias), 1 if accumulate else 0, _ptr(status), ws.data_ptr(), nbytes)
+          _ptr(out_bias), 1 if accumulate else 0, _status(status), ws.data_ptr(), nbytes)
     return out, out_bias
 
 
@@ -358,7 +366,7 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     mean = saved.data.data_ptr()
     _call("ifk_layernorm_backward", dev, dy.data_ptr(), ld, dt, x, ldx, xdt, *q, mean, mean + 4 * rows, _ptr(weight),
-          wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _ptr(status), _ptr(ws), nbytes)
+          wdt, rows, n, dx.data_ptr(), n, _ptr(dw), _ptr(db), _status(status), _ptr(ws), nbytes)
     return dx, dw, db
 
 

@@ -33,6 +33,8 @@ struct BwdArgs {
   const void* w;
   void* dx;
   float* part;  // [2][blocks][n]: the blocks' sums of dy z and of dy; null: not wanted
+  float* dw;    // where the sums go if one block has them all
+  float* db;
   int64_t lddy, ldx, ldc, lds, lddx, rows;
   int n;
   bool w_bf16;
@@ -64,8 +66,10 @@ __device__ __forceinline__ void write_sums(const BwdArgs& a, int team, int c0, i
   for (int c = threadIdx.x; c < 2 * a.n; c += blockDim.x) {
     float v = sums[c];
     for (int q = 1; q < a.teams; ++q) v += sums[(size_t)q * 2 * a.n + c];
-    const int which = c >= a.n;
-    a.part[((int64_t)which * gridDim.x + blockIdx.x) * a.n + (c - which * a.n)] = v;
+    const int which = c >= a.n, col = c - which * a.n;
+    float* out = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.n;
+    if (gridDim.x == 1) out = which ? a.db : a.dw;
+    if (out) out[col] = v;
   }
 }
 size_t sums_bytes(const BwdArgs& a) { return a.part ? (size_t)a.teams * 2 * a.n * sizeof(float) : 0; }
@@ -509,6 +513,8 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
   a.w = w;
   a.dx = dx;
   a.part = (dw || db) ? part : nullptr;
+  a.dw = dw;
+  a.db = db;
   a.lddy = lddy;
   a.ldx = ldx;
   a.ldc = ldc;
@@ -525,6 +531,7 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
   else rc = y_dtype == IFK_F32 ? backward_any<B, float>(a, s) : backward_any<B, B>(a, s);
   if (rc != IFK_OK || !a.part) return rc;
   const int64_t parts = parts_of(rows, n);
+  if (parts == 1 && row_warps(n) <= MAX_W) return IFK_OK;  // the one block has written them
   return sum_parts_run(part, parts, n, dw, part + parts * n, db, 0, s);
 }
 

@@ -483,7 +483,7 @@ IFK_API int ifk_update_bias(float* b, const float* nat_b, int64_t count, double 
  * code * 2^e.  The error is at most 2^e <= a / 64 (half of that where the code
  * is not clipped), and a value has at most 7 significant bits, so it is exact in
  * bf16 and fp32.  A group with a NaN or an infinity has scale byte 255 and codes
- * 0: all its values read as NaN.
+ * 0: all its values read as NaN.  Scale bytes are 1 .. 248, or 255.
  *
  * codes is rows x ld_codes int8 with ld_codes >= ifk_q8_pitch(n) (n rounded up
  * to a multiple of 32; the columns past n are written as 0 and never used), a
@@ -522,7 +522,8 @@ IFK_API size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in,
  * them.  The products are exact and summed in fp32 in either delta type (an fp32
  * delta is taken apart into three bf16 terms); the result does not depend on
  * the run.  rows == 0 gives zeros (or adds nothing).  *d_status (may be NULL)
- * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up.
+ * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; dW and db are
+ * then not valid.  dW and db must not overlap the inputs.
  */
 IFK_API int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int8_t* codes,
                          int64_t ld_codes, const uint8_t* scales, int64_t ld_scales, int64_t rows,
@@ -537,7 +538,7 @@ IFK_API int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, c
  * n values of w_dtype, or are NULL (1 and 0).  mean and rstd (rows fp32) receive
  * the statistics (NULL: not stored).  With codes and scales (both or neither),
  * the 8-bit rows of x are written in the same pass, bit for bit those of
- * ifk_q8_quantize.
+ * ifk_q8_quantize.  y must not overlap x.
  */
 IFK_API int ifk_layernorm(const void* x, int64_t ld_x, int x_dtype, const void* w, const void* b,
                           int w_dtype, int64_t rows, int64_t n, double eps, void* y, int64_t ld_y,

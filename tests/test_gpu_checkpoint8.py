@@ -412,3 +412,34 @@ def test_python_refusals():
     _, s = c8().layer_norm_forward(x, save=True)
     with pytest.raises(ValueError):
         c8().layer_norm_backward(x[:5], s)
+    for bad in (torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(TypeError):
+            c8().quantize_rows(x, status=bad)
+    with pytest.raises(RuntimeError):
+        c8().quantize_rows(x[:0], index=torch.zeros(3, dtype=torch.int64, device="cuda"))  # rows of nothing
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap on the GPU share nothing: each has its own workspace."""
+    rows, n, m = 2600, 512, 384
+    xs = [buffer(rows, n, BF, seed=k) for k in range(2)]
+    ds = [buffer(rows, m, BF, seed=10 + k) for k in range(2)]
+    w = torch.ones(n, device="cuda")
+
+    def work(k):
+        y, s = c8().layer_norm_forward(xs[k], w, None, save=True, checkpoint=True)
+        q = c8().quantize_rows(y)
+        return (y, *c8().layer_norm_backward(xs[1 - k], s, w), *c8().weight_grad(ds[k], q, bias=True))
+
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(work(k))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(p, q) for p, q in zip(out, want[k]))
