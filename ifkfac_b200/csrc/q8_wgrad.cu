@@ -432,12 +432,15 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
           float* p = d + c * ld;
           if (!in) continue;
           if (c + 32 <= cols) {
+            // four addresses, so that the next one does not wait for the last
+            float* at[4] = {p, p + ld, p + 2 * ld, p + 3 * ld};
+            const int64_t ld4 = 4 * ld;
             if (add) {
 #pragma unroll
-              for (int q = 0; q < 32; ++q, p += ld) red_add(p, v[q]);
+              for (int q = 0; q < 32; ++q, at[(q + 3) & 3] += ld4) red_add(at[q & 3], v[q]);
             } else {
 #pragma unroll
-              for (int q = 0; q < 32; ++q, p += ld) *p = v[q];
+              for (int q = 0; q < 32; ++q, at[(q + 3) & 3] += ld4) *at[q & 3] = v[q];
             }
           } else {
 #pragma unroll
