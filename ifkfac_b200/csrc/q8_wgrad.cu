@@ -784,7 +784,8 @@ int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const fl
   cfg.attrs = at;
   cfg.numAttrs = 1;
   IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel, dm, cm, a));
-  const int64_t joins = a.p.total && a.p.Gs > 1 ? a.p.total / a.p.Kt * (TN / JOIN_COLS) : 0;
+  // no tile is cut when the rest divides into whole tiles
+  const int64_t rest = a.p.total / a.p.Kt, joins = rest % a.p.Gs ? rest * (TN / JOIN_COLS) : 0;
   const int64_t blocks = joins + (db ? cdiv(a.n_out, 32) : 0);
   if (blocks) finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(a, (int)joins, sums, parts, delta, ldd, db);
   IFK_CUDA_TRY(cudaGetLastError());
