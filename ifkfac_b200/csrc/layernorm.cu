@@ -2,11 +2,15 @@
 //
 // One pass bound by memory: x is read once into registers (as it is in memory, so a
 // bf16 row takes half of them), the statistics are two sums over the registers, and y
-// (and the 8-bit rows of x) are written.  A team of W warps holds a row, V neighbouring
-// columns a lane at a time: 16 bytes of the wider of x and y, or one element where
-// a row is not aligned for that.  A lane holds up to 32 columns, 64 or 128 bytes in flight,
-// so 16 warps an SM cover the memory's latency; a row no wider than one warp holds needs
-// no barrier.
+// (and the 8-bit rows of x) are written.  A team of W warps holds a row, four neighbouring
+// columns a lane at a time, or one where a row is not aligned for that; a lane holds up to
+// 32.  Four, also where eight bf16 are one 16-byte access: a warp's reads of the fp32
+// weight and bias are then contiguous, and they, from L1, are most of what the load unit
+// does (16384 x 4096 bf16: 51 us against 58; with 8-bit rows, where eight halve the
+// groups' shuffles, 76 against 70, but the sums' order, and so y, would depend on whether
+// the rows are kept).  A row no wider than one warp holds needs no barrier.  Measured:
+// 32768 x 1280 fp32 to bf16 41 us (6.1 TB/s), 16384 x 4096 bf16 51 us (5.3 TB/s),
+// 65536 x 768 fp32 to bf16 with 8-bit rows 62 us (5.7 TB/s).
 #include <algorithm>
 #include <cstring>
 
@@ -46,13 +50,18 @@ __device__ __forceinline__ float team_sum(float v, int W, float* buf) {
   return r;
 }
 
-// 8-bit rows of x, written as ifk_q8_quantize writes them.
+// 8-bit rows of x, written as ifk_q8_quantize writes them: a lane's V columns of a group with the maximum m.
 template <int V>
-__device__ __forceinline__ void write_codes(int8_t* codes, uint8_t* scales, int pitch, int c, const float (&v)[V]) {
-  const uint32_t m = q8::group_max_bits<V>(v), s = q8::scale_byte(m);
+__device__ __forceinline__ void write_group(int8_t* codes, uint8_t* scales, int pitch, int c, const float (&v)[V],
+                                            uint32_t m) {
   if (c >= pitch) return;
+  const uint32_t s = q8::scale_byte(m);
   q8::store_codes<V>(codes + c, v, m, s);
   if ((c & (q8::GROUP - 1)) == 0) scales[c / q8::GROUP] = (uint8_t)s;
+}
+template <int V>
+__device__ __forceinline__ void write_codes(int8_t* codes, uint8_t* scales, int pitch, int c, const float (&v)[V]) {
+  write_group<V>(codes, scales, pitch, c, v, q8::group_max_bits<V>(v));
 }
 
 // The mean is taken twice: the second sum, over x less the first mean, carries what the
@@ -95,12 +104,12 @@ __device__ __forceinline__ void write_out(const FwdArgs& a, TY* y, int c, const 
 // WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
 template <int WARPS>
 constexpr int max_threads() { return WARPS == 0 ? 512 : WARPS == 1 ? 32 * ROWS_PER_BLOCK : 32 * WARPS; }
-// 64 registers a thread, 85 with 64 columns.
-template <int WARPS, int COLS>
-constexpr int min_blocks() { return (COLS > 32 ? 768 : 1024) / max_threads<WARPS>(); }
+// 64 registers a thread.
+template <int WARPS>
+constexpr int min_blocks() { return 1024 / max_threads<WARPS>(); }
 
 template <typename TX, typename TY, int V, int NV, bool PLAIN, int WARPS>
-__global__ void __launch_bounds__(max_threads<WARPS>(), min_blocks<WARPS, V * NV>()) forward_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(max_threads<WARPS>(), min_blocks<WARPS>()) forward_kernel(const FwdArgs a) {
   __shared__ float buf[3][32];
   const int W = WARPS ? WARPS : a.W, lane = threadIdx.x & 31;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * ROWS_PER_BLOCK + (threadIdx.x >> 5) : blockIdx.x;
@@ -195,13 +204,28 @@ __global__ void __launch_bounds__(max_threads<WARPS>(), min_blocks<WARPS, V * NV
   }
   int8_t* codes = a.codes + row * a.ldc;
   uint8_t* scales = a.scales + row * a.lds;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = c0 + k * step;
+  if constexpr (NV == 1) {
     float v[V];
-    unpack(r[k], v);
-    if (a.codes) write_codes<V>(codes, scales, a.pitch, c, v);
-    if (c < a.n) write_out<TY, V, PLAIN>(a, y, c, v, t);
+    unpack(r[0], v);
+    if (a.codes) write_codes<V>(codes, scales, a.pitch, c0, v);
+    if (c0 < a.n) write_out<TY, V, PLAIN>(a, y, c0, v, t);
+  } else {
+    static_assert(NV % 2 == 0, "accesses are handled in pairs");
+#pragma unroll
+    for (int k = 0; k < NV; k += 2) {
+      const int c = c0 + k * step;
+      float v[V], u[V];
+      unpack(r[k], v);
+      unpack(r[k + 1], u);
+      if (a.codes) {
+        uint32_t mv, mu;
+        q8::group_max_bits_of_two<V>(v, u, mv, mu);
+        write_group<V>(codes, scales, a.pitch, c, v, mv);
+        write_group<V>(codes, scales, a.pitch, c + step, u, mu);
+      }
+      if (c < a.n) write_out<TY, V, PLAIN>(a, y, c, v, t);
+      if (c + step < a.n) write_out<TY, V, PLAIN>(a, y, c + step, u, t);
+    }
   }
 }
 
@@ -261,11 +285,11 @@ void launch(FwdArgs& a, cudaStream_t s) {
     forward_kernel<TX, TY, V, NV, PLAIN, 0><<<rows, 32 * a.W, 0, s>>>(a);
 }
 
-// Accesses a lane makes of a row: 32 columns' at most, 64 where both sides are bf16; fewer, by more warps a row, while the rows alone
-// do not give each SM eight warps.
+// Accesses a lane makes of a row: 32 columns' at most; fewer, by more warps a row, while the rows
+// alone do not give each SM eight warps.
 template <typename TX, typename TY, int V>
 int forward(FwdArgs& a, cudaStream_t s) {
-  constexpr int MAXV = V == 8 ? 8 : 32 / V;
+  constexpr int MAXV = 32 / V;
   const int acc = a.pitch / V;  // accesses of a row (with the padding of its last group)
   int W = (int)cdiv(acc, 32 * MAXV);
   if (W > 16) {
@@ -301,10 +325,9 @@ int forward(FwdArgs& a, cudaStream_t s) {
 
 template <typename TX, typename TY>
 int forward_any(FwdArgs& a, cudaStream_t s) {
-  constexpr int V = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
-  const bool al = rows_allow<TX>(a.x, a.ldx, V) && rows_allow<TY>(a.y, a.ldy, V) &&
-                  ((((uintptr_t)a.w) | ((uintptr_t)a.b)) & 15) == 0;
-  return al ? forward<TX, TY, V>(a, s) : forward<TX, TY, 1>(a, s);
+  const bool four = rows_allow<TX>(a.x, a.ldx, 4) && rows_allow<TY>(a.y, a.ldy, 4) &&
+                    ((((uintptr_t)a.w) | ((uintptr_t)a.b)) & 15) == 0;
+  return four ? forward<TX, TY, 4>(a, s) : forward<TX, TY, 1>(a, s);
 }
 
 }  // namespace

@@ -211,6 +211,24 @@ __device__ __forceinline__ uint32_t group_max_bits(const float (&x)[V]) {
   return __float_as_uint(a) & 0x7fffffffu;
 }
 
+// Those of two groups at once, cut to their upper 16 bits: all that the scale and the clipping look at
+// (the order of non-negative numbers is that of their upper bits too).
+template <int V>
+__device__ __forceinline__ void group_max_bits_of_two(const float (&x)[V], const float (&y)[V], uint32_t& mx_x,
+                                                      uint32_t& mx_y) {
+  float a = fabsf(x[0]), b = fabsf(y[0]);
+#pragma unroll
+  for (int i = 1; i < V; ++i) {
+    a = max_nan(a, fabsf(x[i]));
+    b = max_nan(b, fabsf(y[i]));
+  }
+  uint32_t m = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632) & 0x7fff7fffu;
+#pragma unroll
+  for (int o = 1; o < GROUP / V; o *= 2) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  mx_x = m << 16;
+  mx_y = m & 0xffff0000u;
+}
+
 // V codes of a group with this largest magnitude and scale byte to memory (V-byte aligned).
 template <int V>
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&x)[V], uint32_t amax_bits, uint32_t s) {
