@@ -6,7 +6,8 @@
 // then 16 bytes, too; 37 against 40 us for 16384 x 4096), or one element where its rows
 // are not aligned for that (a warp then still covers whole lines).  32 / V neighbouring lanes make a group,
 // so the group's maximum is a few shuffles, and a thread has UNROLL accesses in flight
-// before it uses the first.
+// before it uses the first.  Measured, 16384 x 4096 bf16: to 8 bits 37 us, back 31 to 34 us (203 MB each,
+// 5.5 and 6.2 TB/s; a plain copy of this card runs at 6.5).  Small calls are the launch: 2 us on the device.
 #include <algorithm>
 #include <cstring>
 

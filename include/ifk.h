@@ -5,7 +5,10 @@
  * end (Gsend/ifkfac): the streaming TSQR that folds captured activations X and
  * back-propagated gradients delta into upper-triangular factors R_X / R_G, the
  * damping fold, the four triangular solves that give the natural gradient,
- * and the momentum / lr update of fp32 master weights.
+ * and the momentum / lr update of fp32 master weights.  Beside it stand the
+ * operators a training step with 8-bit activations needs: rows to 8 bits and
+ * back, the weight gradient of a linear layer from such rows, and layer norm
+ * with its backward pass.
  *
  * Conventions
  *  - All matrices are device pointers, row-major, with an explicit leading
