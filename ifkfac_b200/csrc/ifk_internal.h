@@ -196,8 +196,5 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
                            const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const float* mean,
                            const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n, void* dx,
                            int64_t lddx, float* dw, float* db, float* part, int* status, cudaStream_t s);
-// out = sum over the parts of part (parts x n), in a fixed order; likewise part2 into out2 (a null out is skipped)
-int sum_parts_run(const float* part, int64_t parts, int64_t n, float* out, const float* part2, float* out2,
-                  int accumulate, cudaStream_t s);
 
 }  // namespace ifk

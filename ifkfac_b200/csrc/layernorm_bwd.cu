@@ -470,7 +470,7 @@ int backward_any(BwdArgs& a, cudaStream_t s) {
 // out[c] = sum over p of part[p][c] in a fixed order: 32 threads a column take every
 // 32nd p, then one adds the 32.
 __global__ void __launch_bounds__(1024) sum_parts_kernel(const float* part, int64_t parts, int64_t n, float* out,
-                                                         const float* part2, float* out2, int accumulate) {
+                                                         const float* part2, float* out2) {
   __shared__ float sh[32][33];
   const float* src = blockIdx.y ? part2 : part;
   float* dst = blockIdx.y ? out2 : out;
@@ -484,18 +484,10 @@ __global__ void __launch_bounds__(1024) sum_parts_kernel(const float* part, int6
   // the 32 sums of a column, one to a lane
   v = warp_sum(sh[threadIdx.x][threadIdx.y]);
   const int64_t o = (int64_t)blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && o < n) dst[o] = accumulate ? dst[o] + v : v;
+  if (threadIdx.x == 0 && o < n) dst[o] = v;
 }
 
 }  // namespace
-
-int sum_parts_run(const float* part, int64_t parts, int64_t n, float* out, const float* part2, float* out2,
-                  int accumulate, cudaStream_t s) {
-  const dim3 grid((unsigned)cdiv(n, 32), part2 ? 2 : 1);
-  sum_parts_kernel<<<grid, dim3(32, 32), 0, s>>>(part, parts, n, out, part2, out2, accumulate);
-  IFK_CUDA_TRY(cudaGetLastError());
-  return IFK_OK;
-}
 
 size_t layernorm_backward_bytes(int64_t rows, int64_t n) {
   return (size_t)std::max<int64_t>(parts_of(rows, n), 1) * (size_t)n * 2 * sizeof(float);
@@ -534,7 +526,9 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
   if (rc != IFK_OK || !a.part) return rc;
   const int64_t parts = parts_of(rows, n);
   if (parts == 1 && row_warps(n) <= MAX_W) return IFK_OK;  // the one block has written them
-  return sum_parts_run(part, parts, n, dw, part + parts * n, db, 0, s);
+  sum_parts_kernel<<<dim3((unsigned)cdiv(n, 32), 2), dim3(32, 32), 0, s>>>(part, parts, n, dw, part + parts * n, db);
+  IFK_CUDA_TRY(cudaGetLastError());
+  return IFK_OK;
 }
 
 }  // namespace ifk

@@ -96,6 +96,7 @@ struct Args {
   int accumulate;
   bool vec_scales;     // rows of scales start at multiples of 4 bytes
   bool vec_out;        // rows of dW start at multiples of 16 bytes
+  bool copied;         // delta's terms are written by the pass before
   bool whole;          // delta's map has 64-column blocks as a dimension (n_out a multiple of 64)
   int* status;
 };
@@ -195,6 +196,13 @@ __device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// The kernels of a call follow one another; one that is launched behind the last (programmatic stream
+// serialisation) may start and set itself up once every block of the last has run let_next_start or has ended, and
+// wait_for_last holds it until the last is done and its writes are visible.  Each waits before it ends, so the
+// end of a call's last kernel is the end of all of them; the first is launched as usual, after all before it.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void red_add(float* p, float v) {
   asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory");
 }
@@ -290,6 +298,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
       Ring<NS> r;
       const uint32_t bar0 = in_leader(ready);
       bool ok = true, now = true;
+      if (a.copied) wait_for_last();
       while (ok && walk.next(w)) {
         const int o = w.tile / a.p.Ti * TN + (int)rank * (TN / 2);
         for (int k = w.k0; k < w.k1; ++k) {
@@ -520,6 +529,8 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
       }
     }
   }
+  let_next_start();
+  if (threadIdx.x == 0) wait_for_last();
   __syncwarp();
   __syncthreads();
   sync_pair();
@@ -536,6 +547,7 @@ constexpr int FEW_ROWS = 64;  // up to here a pass over delta of its own would c
 __global__ void __launch_bounds__(256)
 finish_kernel(const Args a, int joins, const float* sums, int parts, const __nv_bfloat16* delta, int64_t ldd,
               float* db) {
+  wait_for_last();
   if ((int)blockIdx.x >= joins) {
     __shared__ float sh[8][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -664,6 +676,7 @@ delta_pass_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part, __
       }
     }
   }
+  let_next_start();
   if (!part) return;
   for (int q = 0; q < 8; ++q) {
     __syncthreads();
@@ -770,7 +783,7 @@ bool codes_map(CUtensorMap* m, const int8_t* c, int64_t ld, int64_t rows, int64_
 }
 
 int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const float* sums, int parts,
-           const __nv_bfloat16* delta, int64_t ldd, float* db, cudaStream_t s) {
+           const __nv_bfloat16* delta, int64_t ldd, float* db, bool behind, cudaStream_t s) {
   static thread_local int done_dev = -1;
   int dev = 0;
   IFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -778,23 +791,34 @@ int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const fl
     IFK_CUDA_TRY(cudaFuncSetAttribute(wgrad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     done_dev = dev;
   }
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.p.G * 2));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.attrs = behind ? at : at + 1;
+  cfg.numAttrs = behind ? 2 : 1;
   IFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, wgrad_kernel, dm, cm, a));
   // no tile is cut when the rest divides into whole tiles
   const int64_t rest = a.p.total / a.p.Kt, joins = rest % a.p.Gs ? rest * (TN / JOIN_COLS) : 0;
   const int64_t blocks = joins + (db ? cdiv(a.n_out, 32) : 0);
-  if (blocks) finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(a, (int)joins, sums, parts, delta, ldd, db);
-  IFK_CUDA_TRY(cudaGetLastError());
+  if (blocks) {
+    // behind the products' launch only without shares to join: one row of 2048 x 8192 23 -> 20.5 us, but with
+    // them (1001 x 521 x 1030 fp32) 31 -> 35 us
+    cudaLaunchConfig_t fin{};
+    fin.gridDim = dim3((unsigned)blocks);
+    fin.blockDim = dim3(256);
+    fin.stream = s;
+    fin.attrs = at;
+    fin.numAttrs = joins ? 0 : 1;
+    IFK_CUDA_TRY(cudaLaunchKernelEx(&fin, finish_kernel, a, (int)joins, sums, parts, delta, ldd, db));
+  }
   return IFK_OK;
 }
 
@@ -822,7 +846,9 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.vec_out = ((uintptr_t)dW & 15) == 0 && ldw % 4 == 0;
   a.vec_scales = ((uintptr_t)scales & 3) == 0 && lds % 4 == 0;
   a.status = status;
+  a.copied = l.copy;
   const int parts = (int)sum_splits(rows, n_out);
+  const bool pass = l.copy || (db && rows > FEW_ROWS);
   const void* src = delta;
   int64_t ld = ldd;
   if (l.copy) {
@@ -830,7 +856,7 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
     IFK_CUDA_TRY(cudaGetLastError());
     src = terms;
     ld = l.ldo;
-  } else if (db && rows > FEW_ROWS) {
+  } else if (pass) {
     delta_pass<TD, false>(delta, ldd, rows, n_out, parts, sums, nullptr, 0, s);
     IFK_CUDA_TRY(cudaGetLastError());
   }
@@ -839,7 +865,7 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   if (!delta_map(&dm, src, ld, rows, n_out, l.terms, a.whole) || !codes_map(&cm, codes, ldc, rows, n_in))
     return IFK_ERR_SHAPE;
   const bool few = !l.copy && rows <= FEW_ROWS;  // delta is bf16 then
-  return launch(dm, cm, a, sums, parts, few ? (const __nv_bfloat16*)(const void*)delta : nullptr, ldd, db, s);
+  return launch(dm, cm, a, sums, parts, few ? (const __nv_bfloat16*)(const void*)delta : nullptr, ldd, db, pass, s);
 }
 
 }  // namespace
