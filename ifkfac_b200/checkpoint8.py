@@ -437,8 +437,8 @@ class Linear8(nn.Linear):
         q = None
         if torch.is_grad_enabled() and self.weight.requires_grad:
             q = quantize_rows(x.detach().reshape(-1, x.shape[-1]))
-            if self._share_rows:
-                self._last_rows = q
+        if self._share_rows:
+            self._last_rows = q  # None as well: rows that no hook has taken are not this pass's
         return _LinearQ8.apply(x, self.weight, self.bias, dtype, q)
 
 

@@ -183,6 +183,21 @@ def test_paused_hooks_keep_no_rows():
     hooks.remove()
 
 
+def test_rows_that_no_hook_took_are_not_the_next_passs():
+    """forward() called past the hooks leaves its rows; a pass without gradients has none of its own."""
+    hooks_mod, c8, engine = mods()
+    model = nn.Sequential(c8.Linear8(64, 32, device="cuda"))
+    hooks = hooks_mod.RawActivationHooks(model, batched=True, capture_8bit=True)
+    hooks.enable()
+    first, second = randn(40, 64, seed=1), randn(24, 64, seed=2)
+    model[0].forward(first)
+    with torch.no_grad():
+        model(second)
+    kept, = hooks._pending_X[model[0]]
+    assert torch.equal(kept.unpack(F4).x.double(), rounded(second))
+    hooks.remove()
+
+
 def test_conv_inputs_stay_images():
     AH, _, engine = mods()
     model = nn.Sequential(nn.Conv2d(3, 8, 3, padding=1), nn.Flatten(), nn.Linear(8 * 36, 5)).cuda()
