@@ -22,6 +22,7 @@ Everything runs in libifk.so on CUDA tensors (fp32 or bf16); there is no CPU pat
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -70,6 +71,12 @@ def _call(name: str, dev: int, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise IFKError(rc, name)
+
+
+@lru_cache(maxsize=1024)
+def _workspace(name: str, *sizes: int) -> int:
+    """Bytes that the library's ``name`` asks for (they depend on the sizes alone)."""
+    return getattr(_lib.lib(), name)(*sizes)
 
 
 def _rows2d(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
@@ -256,7 +263,7 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
             out_bias = torch.empty(n_out, dtype=torch.float32, device=dev)
     elif out_bias.dtype != torch.float32 or out_bias.shape != (n_out,) or not out_bias.is_contiguous():
         raise ValueError(f"out_bias must be a contiguous float32 tensor of {n_out}")
-    nbytes = _lib.lib().ifk_q8_wgrad_workspace(rows, n_out, n_in, dt)
+    nbytes = _workspace("ifk_q8_wgrad_workspace", rows, n_out, n_in, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call("ifk_q8_wgrad", dev, delta.data_ptr(), ld, dt, *q.args(), rows, n_out, n_in, out.data_ptr(), ld_out,
           _ptr(out_bias), 1 if accumulate else 0, _status(status), ws.data_ptr(), nbytes)
@@ -362,7 +369,7 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
     if weight_grads:
         dw = torch.empty(n, dtype=torch.float32, device=dev)
         db = torch.empty(n, dtype=torch.float32, device=dev)
-        nbytes = _lib.lib().ifk_layernorm_backward_workspace(rows, n)
+        nbytes = _workspace("ifk_layernorm_backward_workspace", rows, n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     mean = saved.data.data_ptr()
     _call("ifk_layernorm_backward", dev, dy.data_ptr(), ld, dt, x, ldx, xdt, *q, mean, mean + 4 * rows, _ptr(weight),
