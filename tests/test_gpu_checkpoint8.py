@@ -382,6 +382,43 @@ def test_graph_replays_on_new_values_and_other_streams():
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_weight_gradients_queued_behind_one_another():
+    """A call's kernels overlap their launches: calls in a row without a wait, the inputs overwritten right behind
+    them, and the same in a graph, have the bits of calls one at a time."""
+    jobs = []
+    for k, (rows, n_in, n_out, dt, pad) in enumerate(((1, 96, 2304, BF, 0), (65, 521, 72, F4, 3), (700, 768, 1030, BF, 0),
+                                                      (3000, 48, 513, BF, 3), (64, 2048, 520, BF, 0),
+                                                      (1000, 300, 264, F4, 0))):
+        jobs.append((buffer(rows, n_out, dt, pad, seed=k), c8().quantize_rows(buffer(rows, n_in, F4, seed=k + 50))))
+    want = []
+    for delta, q in jobs:
+        want.append(c8().weight_grad(delta, q, bias=True))
+        torch.cuda.synchronize()
+
+    def same(got):
+        return all(torch.equal(p, t) for a, b in zip(got, want) for p, t in zip(a, b))
+
+    for _ in range(3):
+        got = [c8().weight_grad(delta, q, bias=True) for delta, q in jobs]
+        assert same([(w.clone(), b.clone()) for w, b in got])
+    got = []
+    for delta, q in jobs:
+        d = delta.clone()
+        r = c8().Q8Rows(q.codes.clone(), q.scales.clone(), q.cols)
+        got.append(c8().weight_grad(d, r, bias=True))
+        d.fill_(3.0)
+        r.codes.zero_()
+        r.scales.fill_(1)
+    assert same(got)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [c8().weight_grad(delta, q, bias=True) for delta, q in jobs]
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert same(got)
+
+
 def test_python_refusals():
     x = buffer(6, 64, BF)
     q = c8().quantize_rows(x)
