@@ -30,7 +30,9 @@
 // out, the tile out and into the tensor core, delta's half in and twice out), 765 clocks
 // where the tensor core needs 512.  Measured: 16384 x 4096 x 4096 bf16 435 to 470 us (1.2
 // PFLOP/s at the 1.5 GHz that the card's power allows) and 36 us for db's sums and the
-// join; 8192 x 768 x 2304 35 + 16 us (49 in all); one row of 2048 x 8192 17 us (64 MB written).
+// join; 8192 x 768 x 2304 34 + 16 us (49 in all); one row of 2048 x 8192 17 us (67 MB written);
+// 8192 x 4096 x 4096 fp32 720 to 750 us in all.  A launch's fixed part is about 6 us: set-up 1, the
+// first loads 2, the last accumulator's stores 2, the pair's last meeting 1.
 #include <cuda.h>
 
 #include <algorithm>
