@@ -119,6 +119,8 @@ int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const voi
                            const float* mean, const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n,
                            void* dx, int64_t ld_dx, float* dw, float* db, int* d_status, void* workspace,
                            size_t workspace_bytes, ifk_stream_t stream) {
+  const bool withhold = y_dtype & IFK_DEBUG_WITHHOLD;
+  y_dtype &= ~IFK_DEBUG_WITHHOLD;
   if (rows < 0 || n <= 0 || n > MAX_SIDE) return IFK_ERR_SHAPE;
   if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (w && !dtype_ok(w_dtype))) return IFK_ERR_DTYPE;
   cudaStream_t s = S(stream);
@@ -138,7 +140,7 @@ int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const voi
                      workspace_bytes < ifk_layernorm_backward_workspace(rows, n)))
     return IFK_ERR_WORKSPACE;
   return layernorm_backward_run(dy, ld_dy, y_dtype, x, ld_x, x_dtype, codes, ld_codes, scales, ld_scales, mean, rstd,
-                                w, w_dtype, rows, n, dx, ld_dx, dw, db, (float*)workspace, d_status, s);
+                                w, w_dtype, rows, n, dx, ld_dx, dw, db, (float*)workspace, d_status, withhold, s);
 }
 
 }  // extern "C"

@@ -195,6 +195,7 @@ size_t layernorm_backward_bytes(int64_t rows, int64_t n);
 int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype,
                            const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const float* mean,
                            const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n, void* dx,
-                           int64_t lddx, float* dw, float* db, float* part, int* status, cudaStream_t s);
+                           int64_t lddx, float* dw, float* db, float* part, int* status, bool withhold,
+                           cudaStream_t s);
 
 }  // namespace ifk

@@ -42,6 +42,7 @@ struct BwdArgs {
   bool w_bf16;
   int W, teams, depth;  // warps a row, teams a block, rows of a team's ring
   int* status;
+  bool withhold;  // tests only (IFK_DEBUG_WITHHOLD): the first team's first row never counts as landed
 };
 
 constexpr int COLS = 16;         // columns a lane holds: 32 left too few warps for the registers (120 against 80 us
@@ -162,7 +163,9 @@ __device__ __forceinline__ int weight_at(int c) {
 }
 
 // Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
-// A wait that gives up marks the call and the block goes on (its result is not valid).
+// A thread whose wait gives up waits for no other row, and a team's leader then fetches no other: the
+// barrier's phase is still open, and arming it again would be one arrival too many.  The block goes on
+// to its end, since its warps meet at barriers; what it has not received counts as NaN, in dx and in the sums.
 // WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
 template <typename TX, typename TY, int V, int WARPS, bool Q8>
 __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(const BwdArgs a) {
@@ -184,8 +187,10 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
   const int64_t stride = (int64_t)gridDim.x * a.teams, first = (int64_t)blockIdx.x * a.teams + team;
   if (threadIdx.x == 0) failed = 0;
   if (leader) {
+    const int extra = a.withhold && blockIdx.x == 0 && team == 0;
     for (int i = 0; i < a.depth; ++i)
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full + 8 * i), "r"(i == 0 ? 1 + extra : 1)
+                   : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
@@ -223,13 +228,16 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
   };
   if (first < a.rows) ahead(first);
   int slot = 0, ph = 0, par = 0;
+  bool ok = true;  // every row so far has landed
   for (int64_t row = first; row < a.rows; row += stride, par ^= 1) {
-    const float mu = mean, rs = rstd;
+    const float mu = mean;
+    float rs = rstd;
     uint8_t s8[Q8 ? NV : 1];
 #pragma unroll
     for (int k = 0; k < (Q8 ? NV : 1); ++k) s8[k] = sc[k];
     if (row + stride < a.rows) ahead(row + stride);
-    wait_bar(full + 8 * slot, ph, &failed);
+    ok = ok && wait_bar(full + 8 * slot, ph, &failed);
+    if (!ok) rs = __int_as_float(0x7fffffff);
     const uint8_t* in = ring + (size_t)slot * bytes;
     F2 g[NV][H], z[NV][H], sx = f2(0.f), sy = f2(0.f);
     const F2 nmu = f2(-mu), rs2 = f2(rs);
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
       }
     }
     // every lane of the team has read the row
-    if (leader && row + a.depth * stride < a.rows) fetch(row + a.depth * stride, slot);
+    if (leader && ok && row + a.depth * stride < a.rows) fetch(row + a.depth * stride, slot);
     if (++slot == a.depth) {
       slot = 0;
       ph ^= 1;
@@ -304,6 +312,10 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
   for (int k = 0; k < NV; ++k) {
     singles(sw[k], w[k]);
     singles(sb[k], b[k]);
+    if (!ok) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[k][i] = b[k][i] = __int_as_float(0x7fffffff);
+    }
   }
   write_sums<V, NV>(a, team, c0, step, w, b, reinterpret_cast<float*>(smem));
 }
@@ -496,7 +508,8 @@ size_t layernorm_backward_bytes(int64_t rows, int64_t n) {
 int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype,
                            const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const float* mean,
                            const float* rstd, const void* w, int w_dtype, int64_t rows, int64_t n, void* dx,
-                           int64_t lddx, float* dw, float* db, float* part, int* status, cudaStream_t s) {
+                           int64_t lddx, float* dw, float* db, float* part, int* status, bool withhold,
+                           cudaStream_t s) {
   BwdArgs a;
   a.dy = dy;
   a.x = x;
@@ -519,6 +532,7 @@ int layernorm_backward_run(const void* dy, int64_t lddy, int y_dtype, const void
   a.w_bf16 = w_dtype == IFK_BF16;
   a.teams = a.depth = 1;
   a.status = status;
+  a.withhold = withhold;
   using B = __nv_bfloat16;
   int rc;
   if (x_dtype == IFK_F32) rc = y_dtype == IFK_F32 ? backward_any<float, float>(a, s) : backward_any<float, B>(a, s);

@@ -66,6 +66,13 @@ extern "C" {
 #define IFK_F32   0
 #define IFK_BF16  1
 
+/* Tests of the failure path only, or-ed to the element type of the incoming
+ * gradient (ifk_layernorm_backward's y_dtype): one arrival is missing on one of
+ * the call's first barriers, so the waits on it run out (two seconds) where the
+ * call has such waits.  The call then leaves IFK_ERR_TIMEOUT in *d_status, and
+ * the device stays usable for the next one. */
+#define IFK_DEBUG_WITHHOLD 256
+
 /* ---- precision modes -------------------------------------------------- */
 #define IFK_PREC_AUTO  0
 #define IFK_PREC_FP32  1
@@ -558,7 +565,8 @@ IFK_API size_t ifk_layernorm_backward_workspace(int64_t rows, int64_t n);
  * x (x_dtype) is the saved input, or NULL with codes and scales: its 8-bit rows.
  * dy has element type y_dtype.  dx must not overlap the inputs.  rows == 0 gives
  * zero dw and db.  The sums over rows have a fixed order.  *d_status (may be
- * NULL) receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up.
+ * NULL) receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; the rows
+ * of dx that this left without their input, and dw and db, are then NaN.
  */
 IFK_API int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const void* x, int64_t ld_x,
                                    int x_dtype, const int8_t* codes, int64_t ld_codes,
