@@ -50,11 +50,11 @@ constexpr int COLS = 16;         // columns a lane holds: 32 left too few warps 
 constexpr int MAX_W = 16;        // warps a row: up to 32 * 16 * 16 = 8192 columns
 constexpr int BLOCK_WARPS = 16;  // 128 registers a thread
 
-// The block's sums over its rows: the teams' go to shared memory (2 n floats a team) and are added in order.
+// The block's sums over its rows: the teams' go to shared memory (2 n floats a team, free by now) and are added
+// in order.
 template <int V, int NV>
 __device__ __forceinline__ void write_sums(const BwdArgs& a, int team, int c0, int step, const float (&sw)[NV][V],
                                            const float (&sb)[NV][V], float* sums) {
-  __syncthreads();
   float* mine = sums + (size_t)team * 2 * a.n;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -163,9 +163,10 @@ __device__ __forceinline__ int weight_at(int c) {
 }
 
 // Rows by bulk copies.  n is a multiple of V, rows of dy and of the saved form are multiples of 16 bytes.
-// A thread whose wait gives up waits for no other row, and a team's leader then fetches no other: the
-// barrier's phase is still open, and arming it again would be one arrival too many.  The block goes on
-// to its end, since its warps meet at barriers; what it has not received counts as NaN, in dx and in the sums.
+// Once a wait has given up no leader of the block fetches another row: the barrier's phase is still open, and
+// arming it again would be one arrival too many.  The block goes on to its end, since its warps meet at
+// barriers, with NaN as the weight's first value: each row's sums read it, and all of dx its sums.  Its own sums become
+// NaN at the end.
 // WARPS: the warps of a row, known when compiled (the columns' addresses are then constants), or 0.
 template <typename TX, typename TY, int V, int WARPS, bool Q8>
 __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(const BwdArgs a) {
@@ -228,16 +229,13 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
   };
   if (first < a.rows) ahead(first);
   int slot = 0, ph = 0, par = 0;
-  bool ok = true;  // every row so far has landed
   for (int64_t row = first; row < a.rows; row += stride, par ^= 1) {
-    const float mu = mean;
-    float rs = rstd;
+    const float mu = mean, rs = rstd;
     uint8_t s8[Q8 ? NV : 1];
 #pragma unroll
     for (int k = 0; k < (Q8 ? NV : 1); ++k) s8[k] = sc[k];
     if (row + stride < a.rows) ahead(row + stride);
-    ok = ok && wait_bar(full + 8 * slot, ph, &failed);
-    if (!ok) rs = __int_as_float(0x7fffffff);
+    if (!wait_bar(full + 8 * slot, ph, &failed)) *weight = __int_as_float(0x7fffffff);
     const uint8_t* in = ring + (size_t)slot * bytes;
     F2 g[NV][H], z[NV][H], sx = f2(0.f), sy = f2(0.f);
     const F2 nmu = f2(-mu), rs2 = f2(rs);
@@ -284,7 +282,8 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
       }
     }
     // every lane of the team has read the row
-    if (leader && ok && row + a.depth * stride < a.rows) fetch(row + a.depth * stride, slot);
+    if (leader && row + a.depth * stride < a.rows && !*(volatile int*)&failed)
+      fetch(row + a.depth * stride, slot);
     if (++slot == a.depth) {
       slot = 0;
       ph ^= 1;
@@ -302,22 +301,28 @@ __global__ void __launch_bounds__(32 * BLOCK_WARPS, 1) backward_ring_kernel(cons
       store_vec<V, true>((TX*)a.dx + row * a.lddx, c, a.n, o);
     }
   }
-  if (failed && leader) {
-    linger();
-    if (a.status) *a.status = IFK_ERR_TIMEOUT;
-  }
-  if (!a.part) return;
-  float w[NV][V], b[NV][V];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    singles(sw[k], w[k]);
-    singles(sb[k], b[k]);
-    if (!ok) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[k][i] = b[k][i] = __int_as_float(0x7fffffff);
+  __syncthreads();
+  const bool bad = failed;
+  const float nan = __int_as_float(0x7fffffff);
+  if (bad) {
+    if (threadIdx.x == 0) {
+      linger();
+      if (a.status) *a.status = IFK_ERR_TIMEOUT;
     }
+    __syncthreads();
   }
-  write_sums<V, NV>(a, team, c0, step, w, b, reinterpret_cast<float*>(smem));
+  if (a.part) {
+    float w[NV][V], b[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      singles(sw[k], w[k]);
+      singles(sb[k], b[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (bad) w[k][i] = b[k][i] = nan;
+    }
+    write_sums<V, NV>(a, team, c0, step, w, b, reinterpret_cast<float*>(smem));
+  }
 }
 
 // Rows too wide for registers: dx by a block that walks its row twice ...
