@@ -69,6 +69,8 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
                  const uint8_t* scales, int64_t ld_scales, int64_t rows, int64_t n_out, int64_t n_in, float* dW,
                  int64_t ld_dW, float* db, int accumulate, int* d_status, void* workspace, size_t workspace_bytes,
                  ifk_stream_t stream) {
+  const bool withhold = delta_dtype & IFK_DEBUG_WITHHOLD;
+  delta_dtype &= ~IFK_DEBUG_WITHHOLD;
   if (!dW) return IFK_ERR_ARG;
   if (rows < 0 || n_out <= 0 || n_in <= 0 || ld_dW < n_in) return IFK_ERR_SHAPE;
   if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return IFK_ERR_SHAPE;
@@ -89,7 +91,7 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
       workspace_bytes < ifk_q8_wgrad_workspace(rows, n_out, n_in, delta_dtype))
     return IFK_ERR_WORKSPACE;
   return q8_wgrad_run(delta, ld_delta, delta_dtype, codes, ld_codes, scales, ld_scales, rows, n_out, n_in, dW, ld_dW,
-                      db, accumulate ? 1 : 0, d_status, (uint8_t*)workspace, s);
+                      db, accumulate ? 1 : 0, d_status, (uint8_t*)workspace, withhold, s);
 }
 
 int ifk_layernorm(const void* x, int64_t ld_x, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,

@@ -187,7 +187,7 @@ int q8_dequantize_run(const int8_t* codes, int64_t ldc, const uint8_t* scales, i
 size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype);
 int q8_wgrad_run(const void* delta, int64_t ldd, int dtype, const int8_t* codes, int64_t ldc, const uint8_t* scales,
                  int64_t lds, int64_t rows, int64_t n_out, int64_t n_in, float* dW, int64_t ldw, float* db,
-                 int accumulate, int* status, uint8_t* ws, cudaStream_t s);
+                 int accumulate, int* status, uint8_t* ws, bool withhold, cudaStream_t s);
 int layernorm_run(const void* x, int64_t ldx, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,
                   int64_t n, double eps, void* y, int64_t ldy, int y_dtype, float* mean, float* rstd, int8_t* codes,
                   int64_t ldc, uint8_t* scales, int64_t lds, cudaStream_t s);

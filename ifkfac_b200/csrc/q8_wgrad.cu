@@ -102,6 +102,7 @@ struct Args {
   bool copied;         // delta's terms are written by the pass before
   bool whole;          // delta's map has 64-column blocks as a dimension (n_out a multiple of 64)
   int* status;
+  bool withhold;       // tests only (IFK_DEBUG_WITHHOLD): the second CTA's first codes never count as landed
 };
 
 // The steps of a tile in order: which block of KS rows, and which of delta's terms.  The terms of
@@ -301,7 +302,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
     // a group's warps; ready: the copies, and both CTAs' warps of a group; free and acc_full: the products;
     // acc_free: both CTAs' reading warps
     int i = lane, arrivals = 4 * 2;
-    if (i < NC) arrivals = 1 + 32;
+    if (i < NC) arrivals = 1 + 32 + (a.withhold && blockIdx.x == 1 && i == 0 ? 1 : 0);
     else if (i < 2 * NC) arrivals = CONV_WARPS;
     else if (i < 2 * NC + NS) arrivals = 1 + CONV_WARPS * 2;
     else if (i < 2 * NC + 2 * NS + 2) arrivals = 1;
@@ -346,7 +347,6 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
           now = test_bar(free + 8 * r.s, r.ph ^ 1);
         }
       }
-      if (!ok) linger();
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
@@ -380,12 +380,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
             mma_pair(acc, ad + tc::doff(3 * 2048), bd + tc::doff(3 * 2048), idesc, 1u);
             commit_pair(bar);
           }
-          commit_pair(acc_full + 8 * buf);
-          if (!ok) {
-            // a wait gave up: leave once the products already issued are done
-            int quiet = 0;
-            wait_bar(acc_full + 8 * buf, bph, &quiet);
-          }
+          if (ok) commit_pair(acc_full + 8 * buf);
           buf ^= 1;
           if (buf == 0) bph ^= 1;
         }
@@ -409,7 +404,6 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
           now = test_bar(codes_free + 8 * r.s, r.ph ^ 1);
         }
       }
-      if (!ok) linger();
     }
   } else if (warp == 3) {
     // the scale bytes of a slot: rows lane and lane + 32, four groups each; a row past the end has zeros
@@ -493,6 +487,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
       bool add = !to_part && a.accumulate;
       for (int c0 = w.k0; c0 < w.k1; c0 = chunk_end(c0, w.k1)) {
         if (!wait_bar(acc_full + 8 * buf, bph, failed)) {
+          if (in) *d = __int_as_float(0x7fffffff);  // a sum that is not whole: NaN in the first row of the piece
           ok = false;
           break;
         }
@@ -589,6 +584,10 @@ wgrad_kernel(const __grid_constant__ CUtensorMap dmap, const __grid_constant__ C
   __syncwarp();
   if (warp == 2 || warp == 3) pair_wait();
   __syncthreads();
+  // a wait gave up, in whichever warp: what is in flight (copies, those of a warp that has issued all of its own too,
+  // and products) ends before the pair parts
+  if (threadIdx.x == 0 && *failed) linger();
+  __syncwarp();
   pair_arrive();
   pair_wait();
   if (threadIdx.x == 0 && *failed && a.status) *a.status = IFK_ERR_TIMEOUT;
@@ -882,7 +881,7 @@ int launch(const CUtensorMap& dm, const CUtensorMap& cm, const Args& a, const fl
 template <typename TD>
 int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
         int64_t rows, int64_t n_out, int64_t n_in, float* dW, int64_t ldw, float* db, int accumulate, int* status,
-        uint8_t* ws, cudaStream_t s) {
+        uint8_t* ws, bool withhold, cudaStream_t s) {
   if (!encoder()) return IFK_ERR_CUDA;
   const int dtype = sizeof(TD) == 2 ? IFK_BF16 : IFK_F32;
   const Layout l = layout(rows, n_out, n_in, dtype, !rows_allow<TD>(delta, ldd, 8));
@@ -903,6 +902,7 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   a.vec_out = ((uintptr_t)dW & 15) == 0 && ldw % 4 == 0;
   a.vec_scales = ((uintptr_t)scales & 3) == 0 && lds % 4 == 0;
   a.status = status;
+  a.withhold = withhold;
   a.copied = l.copy;
   const int parts = (int)sum_splits(rows, n_out);
   const bool pass = l.copy || (db && rows > FEW_ROWS);
@@ -934,12 +934,12 @@ size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
 
 int q8_wgrad_run(const void* delta, int64_t ldd, int dtype, const int8_t* codes, int64_t ldc, const uint8_t* scales,
                  int64_t lds, int64_t rows, int64_t n_out, int64_t n_in, float* dW, int64_t ldw, float* db,
-                 int accumulate, int* status, uint8_t* ws, cudaStream_t s) {
+                 int accumulate, int* status, uint8_t* ws, bool withhold, cudaStream_t s) {
   if (dtype == IFK_F32)
     return run((const float*)delta, ldd, codes, ldc, scales, lds, rows, n_out, n_in, dW, ldw, db, accumulate, status,
-               ws, s);
+               ws, withhold, s);
   return run((const __nv_bfloat16*)delta, ldd, codes, ldc, scales, lds, rows, n_out, n_in, dW, ldw, db, accumulate,
-             status, ws, s);
+             status, ws, withhold, s);
 }
 
 }  // namespace ifk

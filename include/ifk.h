@@ -67,7 +67,7 @@ extern "C" {
 #define IFK_BF16  1
 
 /* Tests of the failure path only, or-ed to the element type of the incoming
- * gradient (ifk_layernorm_backward's y_dtype): one arrival is missing on one of
+ * gradient (ifk_q8_wgrad's delta_dtype, ifk_layernorm_backward's y_dtype): one arrival is missing on one of
  * the call's first barriers, so the waits on it run out (two seconds) where the
  * call has such waits.  The call then leaves IFK_ERR_TIMEOUT in *d_status, and
  * the device stays usable for the next one. */
@@ -532,8 +532,8 @@ IFK_API size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in,
  * them.  The products are exact and summed in fp32 in either delta type (an fp32
  * delta is taken apart into three bf16 terms); the result does not depend on
  * the run.  rows == 0 gives zeros (or adds nothing).  *d_status (may be NULL)
- * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; dW and db are
- * then not valid.  dW and db must not overlap the inputs.
+ * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; dW is then not
+ * valid and holds NaN.  dW and db must not overlap the inputs.
  */
 IFK_API int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int8_t* codes,
                          int64_t ld_codes, const uint8_t* scales, int64_t ld_scales, int64_t rows,
@@ -566,7 +566,7 @@ IFK_API size_t ifk_layernorm_backward_workspace(int64_t rows, int64_t n);
  * dy has element type y_dtype.  dx must not overlap the inputs.  rows == 0 gives
  * zero dw and db.  The sums over rows have a fixed order.  *d_status (may be
  * NULL) receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; the rows
- * of dx that this left without their input, and dw and db, are then NaN.
+ * of dx that its thread block had left to do, and dw and db, are then NaN.
  */
 IFK_API int ifk_layernorm_backward(const void* dy, int64_t ld_dy, int y_dtype, const void* x, int64_t ld_x,
                                    int x_dtype, const int8_t* codes, int64_t ld_codes,

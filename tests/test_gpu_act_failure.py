@@ -69,3 +69,49 @@ def test_layer_norm_backward_that_waits_for_nothing():
                                   0, None, 0, saved.mean.data_ptr(), saved.rstd.data_ptr(), None, _lib.F32, 7, 40,
                                   dx.data_ptr(), 40, None, None, status.data_ptr(), None, 0, stream())
     assert rc == _lib.OK and torch.equal(dx, want[0]) and status.item() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n_in,n_out,dtype", [
+    (300, 200, 130, BF),          # one tile, one pair
+    (1024, 768, 2304, BF),        # tiles cut into shares
+    (700, 300, 520, F4),
+    (2100, 2049, 2570, BF),       # a wave of tiles, and more than one accumulator
+    (2100, 2049, 2570, F4)])
+def test_weight_grad_without_codes(rows, n_in, n_out, dtype):
+    L = _lib.lib()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = c8().quantize_rows(torch.randn(rows, n_in, generator=g, device="cuda"))
+    delta = torch.randn(rows, n_out, generator=g, device="cuda").to(dtype)
+    want = c8().weight_grad(delta, q, bias=True)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    dW, db = torch.zeros_like(want[0]), torch.zeros_like(want[1])
+    nbytes = L.ifk_q8_wgrad_workspace(rows, n_out, n_in, CODE[dtype])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    rc = L.ifk_q8_wgrad(delta.data_ptr(), n_out, CODE[dtype] | _lib.DEBUG_WITHHOLD, *q.args(), rows, n_out, n_in,
+                        dW.data_ptr(), n_in, db.data_ptr(), 0, status.data_ptr(), ws.data_ptr(), nbytes, stream())
+    assert rc == _lib.OK
+    torch.cuda.synchronize()
+    assert status.item() == _lib.ERR_TIMEOUT
+    # the first pair's first tile; a share of it that another pair has is right
+    assert torch.isnan(dW[0, : min(n_in, 256)]).all()
+    assert torch.equal(db, want[1])                    # its sums do not go through the pair
+    far = dW[:, -1]                                    # and tiles of other pairs are whole
+    if n_in > 256 * 3:
+        assert torch.equal(far, want[0][:, -1])
+    status.zero_()
+    again = c8().weight_grad(delta, q, bias=True, status=status)
+    assert all(torch.equal(p, t) for p, t in zip(again, want)) and status.item() == 0
+
+
+def test_the_flag_does_not_hide_other_errors():
+    import ctypes
+    L, fake, flag = _lib.lib(), ctypes.c_void_p(4096), _lib.DEBUG_WITHHOLD
+    bwd = lambda dt, dy=fake: L.ifk_layernorm_backward(dy, 64, dt, fake, 64, _lib.F32, None, 0, None, 0, fake, fake, None,
+                                                       _lib.F32, 4, 64, fake, 64, None, None, None, None, 0, None)
+    assert bwd(_lib.F32 | flag, None) == _lib.ERR_ARG and bwd(9 | flag) == _lib.ERR_DTYPE and bwd(512) == _lib.ERR_DTYPE
+    wgrad = lambda dt, ws=fake: L.ifk_q8_wgrad(fake, 16, dt, fake, 64, fake, 2, 8, 16, 64, fake, 64, None, 0, None, ws,
+                                               1 << 30, None)
+    assert wgrad(_lib.BF16 | flag, None) == _lib.ERR_WORKSPACE and wgrad(5 | flag) == _lib.ERR_DTYPE
+    # it belongs to these two calls: an element type with it is none elsewhere
+    assert L.ifk_q8_quantize(fake, 64, _lib.F32 | flag, None, 8, 8, 64, fake, 64, fake, 2, None, None) == _lib.ERR_DTYPE
