@@ -435,7 +435,8 @@ class Linear8(nn.Linear):
         rows, self._last_rows = self._last_rows, None
         return rows
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        x = input
         _need_cuda(x, self.weight, self.bias)
         dtype = _autocast_dtype() or self.weight.dtype
         _code(dtype)
@@ -491,7 +492,8 @@ class LayerNorm8(nn.LayerNorm):
         new.weight, new.bias, new.training = m.weight, m.bias, m.training
         return new
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        x = input
         if x.shape[-1] != self.normalized_shape[0]:
             raise ValueError(f"input of width {x.shape[-1]} for a layer norm of {self.normalized_shape[0]}")
         dtype = _autocast_dtype() or x.dtype

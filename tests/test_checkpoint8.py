@@ -204,3 +204,10 @@ def test_capture_8bit_needs_a_mode_that_keeps_rows():
     with pytest.raises(ValueError, match="CUDA"):
         model(torch.randn(3, 4))
     hooks.remove()
+
+
+def test_modules_take_their_input_by_name():
+    """nn.Linear and nn.LayerNorm call it `input`; here the call gets as far as the check of the device."""
+    for m in (c8.Linear8(8, 4), c8.LayerNorm8(8)):
+        with pytest.raises(ValueError, match="CUDA"):
+            m(input=torch.randn(2, 8))
