@@ -413,6 +413,19 @@ class _LinearQ8(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
+_HOOKS = tuple(k for k in nn.Module().__dict__ if "_hooks" in k)
+
+
+def _take_over(new: nn.Module, m: nn.Module) -> nn.Module:
+    """``new`` with the parameters, buffers, submodules and attributes of ``m`` (not its hooks)."""
+    for k, v in m.__dict__.items():
+        if k in ("_parameters", "_buffers", "_modules", "_non_persistent_buffers_set"):
+            new.__dict__[k] = v.copy()
+        elif k not in _HOOKS and k != "forward":
+            new.__dict__[k] = v
+    return new
+
+
 class Linear8(nn.Linear):
     """``nn.Linear`` that keeps its input in 8 bits for the weight gradient.
 
@@ -426,10 +439,8 @@ class Linear8(nn.Linear):
 
     @classmethod
     def from_linear(cls, m: nn.Linear) -> "Linear8":
-        """A Linear8 on the parameters of ``m``."""
-        new = cls(m.in_features, m.out_features, bias=m.bias is not None, device="meta")
-        new.weight, new.bias, new.training = m.weight, m.bias, m.training
-        return new
+        """A Linear8 on the parameters of ``m``, with its attributes."""
+        return _take_over(cls(m.in_features, m.out_features, bias=m.bias is not None, device="meta"), m)
 
     def take_rows(self) -> Optional[Q8Rows]:
         rows, self._last_rows = self._last_rows, None
@@ -486,11 +497,9 @@ class LayerNorm8(nn.LayerNorm):
 
     @classmethod
     def from_layer_norm(cls, m: nn.LayerNorm) -> "LayerNorm8":
-        """A LayerNorm8 on the parameters of ``m``."""
-        new = cls(m.normalized_shape, eps=m.eps, elementwise_affine=m.elementwise_affine, bias=m.bias is not None,
-                  device="meta")
-        new.weight, new.bias, new.training = m.weight, m.bias, m.training
-        return new
+        """A LayerNorm8 on the parameters of ``m``, with its attributes."""
+        return _take_over(cls(m.normalized_shape, eps=m.eps, elementwise_affine=m.elementwise_affine,
+                              bias=m.bias is not None, device="meta"), m)
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         x = input
@@ -505,12 +514,13 @@ class LayerNorm8(nn.LayerNorm):
 def convert(model: nn.Module, linear: bool = True, layer_norm: bool = True) -> nn.Module:
     """``model`` with each nn.Linear (``linear``) and each nn.LayerNorm over one dimension
     (``layer_norm``) replaced, in place, by :class:`Linear8` / :class:`LayerNorm8` on
-    the same parameters.  Subclasses, and layers that already carry hooks, are left as
-    they are: convert before an optimizer attaches its hooks.  A model that is itself
-    such a layer is returned replaced."""
+    the same parameters, with the layer's attributes.  Subclasses, layers that already
+    carry hooks of any kind (a call's, a backward pass's, a state dict's) and layers with a
+    ``forward`` of their own are left as they are: convert before an optimizer attaches
+    its hooks.  A model that is itself such a layer is returned replaced."""
 
     def swap(m: nn.Module) -> nn.Module:
-        if m._forward_hooks or m._backward_hooks or m._forward_pre_hooks or m._backward_pre_hooks:
+        if any(m.__dict__.get(k) for k in _HOOKS) or "forward" in m.__dict__:
             return m
         if linear and type(m) is nn.Linear:
             return Linear8.from_linear(m)

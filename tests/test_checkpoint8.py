@@ -211,3 +211,37 @@ def test_modules_take_their_input_by_name():
     for m in (c8.Linear8(8, 4), c8.LayerNorm8(8)):
         with pytest.raises(ValueError, match="CUDA"):
             m(input=torch.randn(2, 8))
+
+
+@pytest.mark.parametrize("make", [lambda: nn.Linear(8, 8), lambda: nn.LayerNorm(8)])
+def test_convert_keeps_what_a_layer_carries(make):
+    plain = make()
+    plain.tag, plain.info = "q", {"k": 1}
+    plain.register_buffer("mask", torch.ones(8))
+    plain.register_buffer("scratch", torch.ones(2), persistent=False)
+    plain.extra = nn.Parameter(torch.zeros(3))
+    plain.weight.requires_grad_(False)
+    plain.eval()
+    keys = list(nn.Sequential(plain).state_dict())
+    model = c8.convert(nn.Sequential(plain))
+    new = model[0]
+    assert type(new) in (c8.Linear8, c8.LayerNorm8) and type(plain) in (nn.Linear, nn.LayerNorm)
+    assert new.tag == "q" and new.info is plain.info and new.mask is plain.mask and new.extra is plain.extra
+    assert list(model.state_dict()) == keys and "scratch" in dict(new.named_buffers())
+    assert new.weight is plain.weight and not new.weight.requires_grad and not new.training
+    new.register_buffer("later", torch.ones(1))              # containers of its own
+    assert "later" not in plain._buffers
+    assert repr(new).startswith(type(new).__name__)
+
+
+@pytest.mark.parametrize("hook", [
+    lambda m: m.register_state_dict_pre_hook(lambda *a: None), lambda m: m._register_state_dict_hook(lambda *a: None),
+    lambda m: m.register_load_state_dict_post_hook(lambda *a: None),
+    lambda m: m._register_load_state_dict_pre_hook(lambda *a: None),
+    lambda m: m.register_forward_pre_hook(lambda *a: None), lambda m: m.register_full_backward_hook(lambda *a: None),
+    lambda m: setattr(m, "forward", lambda x: x)])
+def test_convert_leaves_layers_with_hooks_or_a_forward_of_their_own(hook):
+    for make, cls in ((lambda: nn.Linear(8, 8), nn.Linear), (lambda: nn.LayerNorm(8), nn.LayerNorm)):
+        m = make()
+        hook(m)
+        assert c8.convert(nn.Sequential(m))[0] is m and type(m) is cls
