@@ -887,7 +887,7 @@ def run_c4(args, rank, world, local_rank):
     torch.manual_seed(0)
     model = GPT().to(dev)
     if args.act8:
-        convert(model)
+        convert(model, autocast_norms=True)  # a pre-norm model: Linear layers read the norms
     g = torch.Generator(device=dev).manual_seed(0)
     idx = torch.randint(0, vocab, (batch, seq + 1), generator=g, device=dev)
     x, y = idx[:, :-1], idx[:, 1:]

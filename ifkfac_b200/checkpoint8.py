@@ -487,37 +487,48 @@ class _LayerNormQ8(torch.autograd.Function):
 
 class LayerNorm8(nn.LayerNorm):
     """``nn.LayerNorm`` over the last dimension that keeps its input in 8 bits for the
-    backward pass.  The output has the input's dtype, or the autocast dtype under
-    autocast (the Linear layers that read it would cast it)."""
+    backward pass.  The output has the input's dtype.  Under autocast it has the autocast
+    dtype, which costs nothing where only Linear layers read it (they would cast it), but is
+    a rounding where it is a residual stream itself; with ``autocast_output=False`` it is
+    fp32 there, as nn.LayerNorm's."""
 
-    def __init__(self, normalized_shape, *args, **kwargs):
+    def __init__(self, normalized_shape, *args, autocast_output: bool = True, **kwargs):
         super().__init__(normalized_shape, *args, **kwargs)
+        self.autocast_output = autocast_output
         if len(self.normalized_shape) != 1:
             raise ValueError(f"LayerNorm8 normalises the last dimension, got {tuple(self.normalized_shape)}")
 
     @classmethod
-    def from_layer_norm(cls, m: nn.LayerNorm) -> "LayerNorm8":
+    def from_layer_norm(cls, m: nn.LayerNorm, autocast_output: bool = True) -> "LayerNorm8":
         """A LayerNorm8 on the parameters of ``m``, with its attributes."""
         return _take_over(cls(m.normalized_shape, eps=m.eps, elementwise_affine=m.elementwise_affine,
-                              bias=m.bias is not None, device="meta"), m)
+                              bias=m.bias is not None, device="meta", autocast_output=autocast_output), m)
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         x = input
         if x.shape[-1] != self.normalized_shape[0]:
             raise ValueError(f"input of width {x.shape[-1]} for a layer norm of {self.normalized_shape[0]}")
-        dtype = _autocast_dtype() or x.dtype
+        dtype = _autocast_dtype()
+        if dtype is None:
+            dtype = x.dtype
+        elif not self.autocast_output:
+            dtype = torch.float32
         params = [p for p in (x, self.weight, self.bias) if p is not None]
         save = torch.is_grad_enabled() and any(p.requires_grad for p in params)
         return _LayerNormQ8.apply(x, self.weight, self.bias, self.eps, dtype, save)
 
 
-def convert(model: nn.Module, linear: bool = True, layer_norm: bool = True) -> nn.Module:
+def convert(model: nn.Module, linear: bool = True, layer_norm: bool = True, autocast_norms: bool = False) -> nn.Module:
     """``model`` with each nn.Linear (``linear``) and each nn.LayerNorm over one dimension
     (``layer_norm``) replaced, in place, by :class:`Linear8` / :class:`LayerNorm8` on
     the same parameters, with the layer's attributes.  Subclasses, layers that already
     carry hooks of any kind (a call's, a backward pass's, a state dict's) and layers with a
     ``forward`` of their own are left as they are: convert before an optimizer attaches
-    its hooks.  A model that is itself such a layer is returned replaced."""
+    its hooks.  A model that is itself such a layer is returned replaced.
+
+    Under autocast the layer norms' outputs stay fp32, as nn.LayerNorm's are; with
+    ``autocast_norms`` they have the autocast dtype, for models whose norms only Linear
+    layers read (see :class:`LayerNorm8`)."""
 
     def swap(m: nn.Module) -> nn.Module:
         if any(m.__dict__.get(k) for k in _HOOKS) or "forward" in m.__dict__:
@@ -525,7 +536,7 @@ def convert(model: nn.Module, linear: bool = True, layer_norm: bool = True) -> n
         if linear and type(m) is nn.Linear:
             return Linear8.from_linear(m)
         if layer_norm and type(m) is nn.LayerNorm and len(m.normalized_shape) == 1:
-            return LayerNorm8.from_layer_norm(m)
+            return LayerNorm8.from_layer_norm(m, autocast_norms)
         return m
 
     done = {}
