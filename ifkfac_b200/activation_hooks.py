@@ -139,6 +139,7 @@ class RawActivationHooks:
         self.chunk_transform_X = None
         self.chunk_transform_G = None
         self._handles: List = []
+        self._sharing: List[Linear8] = []  # layers that hand over their rows, once an enable()
         self._enabled = False
         self._fx: Dict[nn.Module, Optional[Factor]] = {}
         self._fg: Dict[nn.Module, Optional[Factor]] = {}
@@ -192,7 +193,8 @@ class RawActivationHooks:
             self._handles.append(module.register_forward_hook(self._forward_hook))
             self._handles.append(module.register_full_backward_hook(self._backward_hook))
             if self.capture_8bit and isinstance(module, Linear8):
-                module._share_rows = True
+                module.share_rows()
+                self._sharing.append(module)
         self._enabled = True
 
     def pause(self) -> None:
@@ -279,7 +281,7 @@ class RawActivationHooks:
 
     # ---- hooks ----
     def _forward_hook(self, module, inp, out):
-        shared = module.take_rows() if isinstance(module, Linear8) else None
+        shared = module.take_rows(out) if self.capture_8bit and isinstance(module, Linear8) else None
         if not self._enabled:
             return
         x = prepare_x(inp[0].detach(), module, self.max_conv_rows, self.max_seq_rows,
@@ -417,9 +419,8 @@ class RawActivationHooks:
         for h in self._handles:
             h.remove()
         self._handles.clear()
-        for module in self._linear_layers:
-            if isinstance(module, Linear8):
-                module._share_rows = False
-                module.take_rows()
+        for module in self._sharing:
+            module.unshare_rows()
+        self._sharing.clear()
         self._enabled = False
         self.clear()

@@ -22,6 +22,7 @@ Everything runs in libifk.so on CUDA tensors (fp32 or bf16); there is no CPU pat
 """
 from __future__ import annotations
 
+import weakref
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -426,25 +427,60 @@ def _take_over(new: nn.Module, m: nn.Module) -> nn.Module:
     return new
 
 
+class _PassRows:
+    """The rows of one forward pass on their way to the hooks: ``left`` sets of hooks have yet to
+    take them, at the call whose output is ``out``.  A copy or a pickle of the layer has none."""
+
+    __slots__ = ("rows", "out", "left")
+
+    def __init__(self, rows: Optional[Q8Rows] = None, out: Optional[torch.Tensor] = None, left: int = 0):
+        self.rows, self.out, self.left = rows, None if out is None else weakref.ref(out), left
+
+    def __reduce__(self):
+        return _PassRows, ()
+
+
 class Linear8(nn.Linear):
     """``nn.Linear`` that keeps its input in 8 bits for the weight gradient.
 
     Forward and input gradient are ``nn.Linear``'s (in the autocast dtype under
     autocast); the weight and bias gradients come from :func:`weight_grad`, summed in
-    fp32.  While hooks that capture in 8 bits are attached, ``take_rows`` hands them
-    the rows of the last forward pass, so they are quantised once."""
+    fp32.  While hooks that capture in 8 bits are attached (``share_rows``), ``take_rows``
+    hands each set of them the rows of the forward pass, so they are quantised once."""
 
-    _share_rows = False   # set by the hooks that want the rows
-    _last_rows: Optional[Q8Rows] = None
+    _share_rows = 0                       # sets of hooks that want the rows
+    _pass: Optional[_PassRows] = None
 
     @classmethod
     def from_linear(cls, m: nn.Linear) -> "Linear8":
         """A Linear8 on the parameters of ``m``, with its attributes."""
         return _take_over(cls(m.in_features, m.out_features, bias=m.bias is not None, device="meta"), m)
 
-    def take_rows(self) -> Optional[Q8Rows]:
-        rows, self._last_rows = self._last_rows, None
-        return rows
+    @property
+    def _last_rows(self) -> Optional[Q8Rows]:
+        """The rows that not every set of hooks has taken yet."""
+        p = self._pass
+        return None if p is None else p.rows
+
+    def share_rows(self) -> None:
+        """One more set of hooks takes the rows of each forward pass ..."""
+        self._share_rows += 1
+
+    def unshare_rows(self) -> None:
+        """... and one no longer does."""
+        self._share_rows = max(self._share_rows - 1, 0)
+        self._pass = None
+
+    def take_rows(self, out: torch.Tensor) -> Optional[Q8Rows]:
+        """The rows of the forward pass whose output is ``out``, for one set of hooks; None when
+        that pass had none, or another one (a thread's) has come since."""
+        p = self._pass
+        if p is None or p.rows is None or p.out() is not out:
+            return None
+        p.left -= 1
+        if p.left <= 0 and self._pass is p:
+            self._pass = None
+        return p.rows
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         x = input
@@ -456,9 +492,11 @@ class Linear8(nn.Linear):
         q = None
         if torch.is_grad_enabled() and self.weight.requires_grad:
             q = quantize_rows(x.detach().reshape(-1, x.shape[-1]))
+        y = _LinearQ8.apply(x, self.weight, self.bias, dtype, q)
         if self._share_rows:
-            self._last_rows = q  # None as well: rows that no hook has taken are not this pass's
-        return _LinearQ8.apply(x, self.weight, self.bias, dtype, q)
+            # none as well: rows that no hook has taken are not this pass's
+            self._pass = None if q is None else _PassRows(q, y, self._share_rows)
+        return y
 
 
 class _LayerNormQ8(torch.autograd.Function):

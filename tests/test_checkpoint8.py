@@ -245,3 +245,53 @@ def test_convert_leaves_layers_with_hooks_or_a_forward_of_their_own(hook):
         m = make()
         hook(m)
         assert c8.convert(nn.Sequential(m))[0] is m and type(m) is cls
+
+
+def _rows(n=4):
+    return c8.Q8Rows(torch.zeros(n, 32, dtype=torch.int8), torch.ones(n, 1, dtype=torch.uint8), 20)
+
+
+def test_a_passs_rows_go_to_the_hooks_of_that_pass():
+    m, q, out, other = c8.Linear8(20, 4), _rows(), torch.zeros(2), torch.zeros(2)
+    m.share_rows()
+    m.share_rows()
+    m._pass = c8._PassRows(q, out, m._share_rows)
+    assert m.take_rows(other) is None and m._last_rows is q  # another pass's output
+    assert m.take_rows(out) is q and m._last_rows is q       # two sets of hooks each take them
+    assert m.take_rows(out) is q and m._last_rows is None
+    assert m.take_rows(out) is None
+    m.unshare_rows()
+    assert m._share_rows == 1
+    m.unshare_rows()
+    m.unshare_rows()
+    assert m._share_rows == 0
+
+
+def test_copies_and_pickles_of_a_layer_hold_no_rows():
+    import copy
+    import io
+    m, out = c8.Linear8(20, 4), torch.zeros(2)
+    m._pass = c8._PassRows(_rows(), out, 1)
+    assert copy.deepcopy(m)._last_rows is None
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    back = torch.load(f, weights_only=False)
+    assert back._last_rows is None and torch.equal(back.weight, m.weight)
+    assert m._last_rows is not None
+
+
+def test_hooks_leave_the_layers_as_they_found_them():
+    from ifkfac_b200.activation_hooks import RawActivationHooks
+    model = c8.convert(nn.Sequential(nn.Linear(4, 4)))
+    sets = [RawActivationHooks(model, capture_8bit=True, batched=True) for _ in range(2)]
+    plain = RawActivationHooks(model, batched=True)
+    for h in (*sets, plain):
+        h.enable()
+    assert model[0]._share_rows == 2
+    plain.remove()
+    sets[0].remove()
+    sets[0].remove()
+    assert model[0]._share_rows == 1                         # the other set still gets its rows
+    sets[1].remove()
+    assert model[0]._share_rows == 0

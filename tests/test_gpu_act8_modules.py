@@ -62,3 +62,92 @@ def test_a_converted_post_norm_block_keeps_its_residual_stream():
     assert want.dtype == got.dtype == F4
     got.sum().backward()
     assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+
+
+def counted(monkeypatch, engine):
+    packed, pack = [], engine.quantize_rows
+    monkeypatch.setattr(engine, "quantize_rows", lambda *a, **k: packed.append(1) or pack(*a, **k))
+    return packed
+
+
+def rounded(x):
+    _, c8, _ = mods()
+    return c8.dequantize_rows(c8.quantize_rows(x.reshape(-1, x.shape[-1])), F4)
+
+
+def test_several_sets_of_hooks_share_a_layers_rows(monkeypatch):
+    """Hooks that do not capture in 8 bits leave the rows to those that do, two sets that do both get
+    them, and one that goes takes nothing from the other."""
+    AH, c8, engine = mods()
+    model = nn.Sequential(c8.Linear8(40, 24, device="cuda"))
+    plain = AH.RawActivationHooks(model, batched=True)
+    one, two = (AH.RawActivationHooks(model, batched=True, capture_8bit=True) for _ in range(2))
+    for h in (plain, one, two):
+        h.enable()
+    packed = counted(monkeypatch, engine)
+    x = randn(50, 40)
+    with torch.no_grad():
+        model(x)                                             # no rows of the layer's own
+    assert len(packed) == 2
+    for h in (one, two):
+        h.clear()
+    del packed[:]
+    y = model(x)
+    assert not packed and model[0]._last_rows is None
+    a, b = one._pending_X[model[0]][0], two._pending_X[model[0]][0]
+    assert a.q is b.q and torch.equal(a.unpack(F4).x, rounded(x))
+    assert isinstance(plain._pending_X[model[0]][0], engine.Rows)
+    y.sum().backward()
+    del packed[:]
+    one.remove()
+    model(x)
+    assert not packed and torch.equal(two._pending_X[model[0]][1].unpack(F4).x, rounded(x))
+    two.remove()
+    plain.remove()
+
+
+def test_rows_of_a_pass_within_another_ones_hooks():
+    """A forward pass of the layer, of as many rows, between a pass and its hooks."""
+    AH, c8, engine = mods()
+    model = nn.Sequential(c8.Linear8(40, 24, device="cuda"))
+    first, second = randn(50, 40, seed=1), randn(50, 40, seed=2)
+    handle = model[0].register_forward_hook(lambda m, i, o: [m.forward(second), None][1])
+    hooks = AH.RawActivationHooks(model, batched=True, capture_8bit=True)
+    hooks.enable()
+    model(first)
+    kept, = hooks._pending_X[model[0]]
+    assert torch.equal(kept.unpack(F4).x, rounded(first))
+    hooks.remove()
+    handle.remove()
+
+
+def test_threads_in_one_layer_keep_their_own_rows():
+    AH, c8, engine = mods()
+    model = nn.Sequential(c8.Linear8(64, 16, device="cuda"))
+    hooks = AH.RawActivationHooks(model, batched=True, capture_8bit=True)
+    got = {}
+    accumulate = hooks._accumulate
+    hooks._accumulate = lambda m, c, *a: (got.setdefault(threading.get_ident(), []).append(c), accumulate(m, c, *a))
+    hooks.enable()
+    xs = [randn(32, 64, seed=k) for k in range(4)]
+    ids, start = {}, threading.Barrier(4)
+
+    def work(k):
+        ids[k] = threading.get_ident()
+        start.wait()
+        for _ in range(25):
+            model(xs[k])
+        start.wait()                                         # no thread's identity is used again
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(4):
+        want = rounded(xs[k])
+        assert len(got[ids[k]]) == 25
+        for c in got[ids[k]]:
+            c = c if isinstance(c, engine.PackedRows) else engine.PackedRows.pack(c)
+            assert torch.equal(c.unpack(F4).x, want)
+    hooks.remove()
