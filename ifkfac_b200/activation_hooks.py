@@ -115,7 +115,7 @@ class RawActivationHooks:
     """
 
     _SEQ_SUBSAMPLE: int = 2048
-    # values unpacked from 8 bits at a time, for one fold call
+    # values unpacked from 8 bits at a time, for one fold call; a chunk (one pass's rows of a layer) is not split
     _UNPACK_BYTES: int = 1 << 30
 
     def __init__(self, model: nn.Module, damping: float = 1e-2, max_out_dim: int = 0,
@@ -243,22 +243,29 @@ class RawActivationHooks:
         mix fp32 and bf16 (each segment carries its type); with PREC_AUTO the
         precision follows the chunk type, so the dtypes fold in separate calls."""
         batch, size = [], 0
-        for e in entries:
-            # rows kept in 8 bits are unpacked for the call that folds them: a share of the entries at a time
-            add = sum(4 * c.rows * c.cols for c in e[2] if isinstance(c, PackedRows))
-            if batch and size + add > self._UNPACK_BYTES:
-                self._fold_batch(batch)
-                batch, size = [], 0
-            batch.append(e)
-            size += add
+        for table, module, chunks in entries:
+            part = []
+            for c in chunks:
+                # rows kept in 8 bits are unpacked for the call that folds them: a share of the chunks at a time
+                add = c.q.rows * c.q.cols * self._unpacked_dtype(c).itemsize if isinstance(c, PackedRows) else 0
+                if add and size and size + add > self._UNPACK_BYTES:
+                    if part:
+                        batch.append((table, module, part))
+                    self._fold_batch(batch)
+                    batch, part, size = [], [], 0
+                part.append(c)
+                size += add
+            if part:
+                batch.append((table, module, part))
         if batch:
             self._fold_batch(batch)
 
+    def _unpacked_dtype(self, c: PackedRows) -> torch.dtype:
+        # exact in either dtype: bf16 unless the precision follows the captured one
+        return c.dtype if self.precision == _lib.PREC_AUTO else torch.bfloat16
+
     def _rows_of(self, c) -> Rows:
-        if isinstance(c, PackedRows):
-            # exact in either dtype: bf16 unless the precision follows the captured one
-            return c.unpack(None if self.precision == _lib.PREC_AUTO else torch.bfloat16)
-        return as_rows(c)
+        return c.unpack(self._unpacked_dtype(c)) if isinstance(c, PackedRows) else as_rows(c)
 
     def _fold_batch(self, entries) -> None:
         groups: Dict[Tuple, List] = {}

@@ -295,3 +295,30 @@ def test_hooks_leave_the_layers_as_they_found_them():
     assert model[0]._share_rows == 1                         # the other set still gets its rows
     sets[1].remove()
     assert model[0]._share_rows == 0
+
+
+@pytest.mark.parametrize("precision,size", [(_lib.PREC_AUTO, 4), (_lib.PREC_BF16, 2), (_lib.PREC_FP32, 2)])
+def test_rows_are_unpacked_a_share_at_a_time(precision, size):
+    """One layer's chunks too: every fold call but one of a single chunk stays under the limit, and each
+    table's chunks stay in their order."""
+    from ifkfac_b200.activation_hooks import RawActivationHooks
+    from ifkfac_b200.engine import PackedRows, Rows
+    hooks = RawActivationHooks(nn.Sequential(nn.Linear(20, 4)), capture_8bit=True, batched=True, precision=precision)
+    calls = []
+    hooks._fold_batch = lambda entries: calls.append(entries)
+    hooks._UNPACK_BYTES = 10 * 20 * size
+    chunks = [PackedRows(_rows(n), torch.float32, ones=True) for n in (3, 4, 2, 2, 50, 1, 9, 9, 1)]
+    plain = Rows(torch.zeros(1000, 20))                      # not unpacked: counts for nothing
+    entries = [("X", "a", chunks[:4]), ("G", "a", [plain] + chunks[4:6]), ("X", "b", chunks[6:])]
+    hooks._fold_entries(entries)
+    for e in calls:
+        assert len({(t, m) for t, m, _ in e}) == len(e) and all(cs for _, _, cs in e)
+        packed = [c for _, _, cs in e for c in cs if isinstance(c, PackedRows)]
+        assert len(packed) == 1 or sum(c.rows * 20 * size for c in packed) <= hooks._UNPACK_BYTES
+    for table, module, want in entries:
+        got = [c for e in calls for t, m, cs in e if (t, m) == (table, module) for c in cs]
+        assert got == want
+    assert len(calls) == 5                                   # 3 4 2 | 2 | 50 | 1 9 | 9 1
+    calls.clear()
+    hooks._fold_entries([("X", "a", [plain] * 3), ("G", "a", [plain])])
+    assert calls == [[("X", "a", [plain] * 3), ("G", "a", [plain])]]
