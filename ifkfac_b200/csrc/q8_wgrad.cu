@@ -715,6 +715,7 @@ delta_pass_kernel(const TD* d, int64_t ldd, int64_t rows, int n, float* part, __
       if (TERMS && r + j * stride < rows && c < ldo) {
         __nv_bfloat16* o = out + (r + j * stride) * ldo + c;
         if constexpr (sizeof(TD) == 2) {
+          static_assert(!TERMS || V == 1, "rows aligned for more are read in place");
           store_vec<V, true>(o, 0, V, v);
         } else {
           float t[3][V];
@@ -752,16 +753,21 @@ int64_t sum_splits(int64_t rows, int64_t n) {
   return std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, 64), SM_COUNT * 4 / cdiv(n, 256)));
 }
 
-template <typename TD, bool TERMS>
+template <typename TD, int V, bool TERMS>
 void delta_pass(const TD* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part, __nv_bfloat16* out,
                 int64_t ldo, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(TD);
-  if (rows_allow<TD>(d, ldd, V))
-    delta_pass_kernel<TD, V, TERMS><<<dim3((unsigned)cdiv(TERMS ? ldo : n, 32 * V), (unsigned)splits), 256, 0, s>>>(
-        d, ldd, rows, (int)n, part, out, ldo);
-  else
-    delta_pass_kernel<TD, 1, TERMS><<<dim3((unsigned)cdiv(TERMS ? ldo : n, 32), (unsigned)splits), 256, 0, s>>>(
-        d, ldd, rows, (int)n, part, out, ldo);
+  delta_pass_kernel<TD, V, TERMS><<<dim3((unsigned)cdiv(TERMS ? ldo : n, 32 * V), (unsigned)splits), 256, 0, s>>>(
+      d, ldd, rows, (int)n, part, out, ldo);
+}
+// fp32 in three terms, or the bf16 rows that TMA cannot read, which are those that are not aligned for 16 bytes.
+void copy_delta(const float* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part, __nv_bfloat16* out,
+                int64_t ldo, cudaStream_t s) {
+  if (rows_allow<float>(d, ldd, 4)) delta_pass<float, 4, true>(d, ldd, rows, n, splits, part, out, ldo, s);
+  else delta_pass<float, 1, true>(d, ldd, rows, n, splits, part, out, ldo, s);
+}
+void copy_delta(const __nv_bfloat16* d, int64_t ldd, int64_t rows, int64_t n, int64_t splits, float* part,
+                __nv_bfloat16* out, int64_t ldo, cudaStream_t s) {
+  delta_pass<__nv_bfloat16, 1, true>(d, ldd, rows, n, splits, part, out, ldo, s);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -909,12 +915,12 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
   const void* src = delta;
   int64_t ld = ldd;
   if (l.copy) {
-    delta_pass<TD, true>(delta, ldd, rows, n_out, parts, db ? sums : nullptr, terms, l.ldo, s);
+    copy_delta(delta, ldd, rows, n_out, parts, db ? sums : nullptr, terms, l.ldo, s);
     IFK_CUDA_TRY(cudaGetLastError());
     src = terms;
     ld = l.ldo;
   } else if (pass) {
-    delta_pass<TD, false>(delta, ldd, rows, n_out, parts, sums, nullptr, 0, s);
+    if constexpr (sizeof(TD) == 2) delta_pass<TD, 8, false>(delta, ldd, rows, n_out, parts, sums, nullptr, 0, s);
     IFK_CUDA_TRY(cudaGetLastError());
   }
   CUtensorMap dm, cm;
