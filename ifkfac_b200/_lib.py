@@ -23,6 +23,7 @@ PREC_AUTO, PREC_FP32, PREC_BF16 = 0, 1, 2
 FOLD_TRAPEZOIDAL_CHUNK = 1
 FOLD_DEBUG_WITHHOLD = 256  # tests of the failure path only
 DEBUG_WITHHOLD = 256  # or-ed to an element type; tests of the failure path only
+DELTA_IN_PLACE = 512  # or-ed to BF16: the weight gradient reads delta in place
 Q8_GROUP = 32
 
 _i64, _sz, _vp, _int, _dbl = ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_int, ctypes.c_double

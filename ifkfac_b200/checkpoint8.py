@@ -264,9 +264,12 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
             out_bias = torch.empty(n_out, dtype=torch.float32, device=dev)
     elif out_bias.dtype != torch.float32 or out_bias.shape != (n_out,) or not out_bias.is_contiguous():
         raise ValueError(f"out_bias must be a contiguous float32 tensor of {n_out}")
+    p = delta.data_ptr()
+    if dt == _lib.BF16 and p % 16 == 0 and ld % 8 == 0:
+        dt |= _lib.DELTA_IN_PLACE  # no copy of delta, and no room for one
     nbytes = _workspace("ifk_q8_wgrad_workspace", rows, n_out, n_in, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call("ifk_q8_wgrad", dev, delta.data_ptr(), ld, dt, *q.args(), rows, n_out, n_in, out.data_ptr(), ld_out,
+    _call("ifk_q8_wgrad", dev, p, ld, dt, *q.args(), rows, n_out, n_in, out.data_ptr(), ld_out,
           _ptr(out_bias), 1 if accumulate else 0, _status(status), ws.data_ptr(), nbytes)
     return out, out_bias
 

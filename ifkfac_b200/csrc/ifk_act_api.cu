@@ -60,9 +60,11 @@ int ifk_q8_dequantize(const int8_t* codes, int64_t ld_codes, const uint8_t* scal
 }
 
 size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in, int delta_dtype) {
+  const bool in_place = delta_dtype == (IFK_BF16 | IFK_DELTA_IN_PLACE);
+  if (in_place) delta_dtype = IFK_BF16;
   if (rows < 0 || n_out <= 0 || n_in <= 0 || !dtype_ok(delta_dtype)) return 0;
   if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return 0;
-  return align_up(q8_wgrad_bytes(rows, n_out, n_in, delta_dtype)) + ALIGN;
+  return align_up(q8_wgrad_bytes(rows, n_out, n_in, delta_dtype, !in_place)) + ALIGN;
 }
 
 int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int8_t* codes, int64_t ld_codes,
@@ -71,6 +73,9 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
                  ifk_stream_t stream) {
   const bool withhold = delta_dtype & IFK_DEBUG_WITHHOLD;
   delta_dtype &= ~IFK_DEBUG_WITHHOLD;
+  const int sized_as = delta_dtype;
+  const bool in_place = delta_dtype == (IFK_BF16 | IFK_DELTA_IN_PLACE);
+  if (in_place) delta_dtype = IFK_BF16;
   if (!dW) return IFK_ERR_ARG;
   if (rows < 0 || n_out <= 0 || n_in <= 0 || ld_dW < n_in) return IFK_ERR_SHAPE;
   if (rows > MAX_SIDE || n_out > MAX_SIDE || n_in > MAX_SIDE) return IFK_ERR_SHAPE;
@@ -85,10 +90,11 @@ int ifk_q8_wgrad(const void* delta, int64_t ld_delta, int delta_dtype, const int
   }
   if (!delta) return IFK_ERR_ARG;
   if (ld_delta < n_out) return IFK_ERR_SHAPE;
+  if (in_place && (((uintptr_t)delta & 15) || ld_delta % 8)) return IFK_ERR_ARG;
   const int rc = q8_rows_ok(codes, ld_codes, scales, ld_scales, n_in);
   if (rc != IFK_OK) return rc;
   if (!workspace || !aligned(workspace) ||
-      workspace_bytes < ifk_q8_wgrad_workspace(rows, n_out, n_in, delta_dtype))
+      workspace_bytes < ifk_q8_wgrad_workspace(rows, n_out, n_in, sized_as))
     return IFK_ERR_WORKSPACE;
   return q8_wgrad_run(delta, ld_delta, delta_dtype, codes, ld_codes, scales, ld_scales, rows, n_out, n_in, dW, ld_dW,
                       db, accumulate ? 1 : 0, d_status, (uint8_t*)workspace, withhold, s);

@@ -184,7 +184,8 @@ int q8_quantize_run(const void* x, int64_t ldx, int dtype, const int64_t* ridx, 
 int q8_dequantize_run(const int8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, const int64_t* ridx,
                       int64_t src_rows, int64_t rows, int64_t n, void* out, int64_t ldo, int dtype, int* status,
                       cudaStream_t s);
-size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype);
+// copy: with room for a bf16 delta whose rows TMA cannot read.
+size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype, bool copy);
 int q8_wgrad_run(const void* delta, int64_t ldd, int dtype, const int8_t* codes, int64_t ldc, const uint8_t* scales,
                  int64_t lds, int64_t rows, int64_t n_out, int64_t n_in, float* dW, int64_t ldw, float* db,
                  int accumulate, int* status, uint8_t* ws, bool withhold, cudaStream_t s);

@@ -933,8 +933,8 @@ int run(const TD* delta, int64_t ldd, const int8_t* codes, int64_t ldc, const ui
 
 }  // namespace
 
-size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
-  const Layout l = layout(rows, n_out, n_in, dtype, true);
+size_t q8_wgrad_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype, bool copy) {
+  const Layout l = layout(rows, n_out, n_in, dtype, copy);
   return l.sums + l.terms_b + l.part;
 }
 

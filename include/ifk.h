@@ -73,6 +73,11 @@ extern "C" {
  * the device stays usable for the next one. */
 #define IFK_DEBUG_WITHHOLD 256
 
+/* Or-ed to IFK_BF16 as the delta type of ifk_q8_wgrad_workspace and ifk_q8_wgrad:
+ * delta's base is a multiple of 16 bytes and ld_delta of 8, so delta is read in
+ * place and the workspace has no room for a copy of it. */
+#define IFK_DELTA_IN_PLACE 512
+
 /* ---- precision modes -------------------------------------------------- */
 #define IFK_PREC_AUTO  0
 #define IFK_PREC_FP32  1
@@ -521,7 +526,8 @@ IFK_API int ifk_q8_dequantize(const int8_t* codes, int64_t ld_codes, const uint8
                               int64_t rows, int64_t n, void* out, int64_t ld_out, int out_dtype,
                               int* d_status, ifk_stream_t stream);
 
-/* Workspace bytes for ifk_q8_wgrad (with or without db). */
+/* Workspace bytes for ifk_q8_wgrad (with or without db), for any alignment of delta's rows; without
+ * the 2 bytes an element of a bf16 delta's copy when delta_dtype is IFK_BF16 | IFK_DELTA_IN_PLACE. */
 IFK_API size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in, int delta_dtype);
 
 /*
@@ -531,7 +537,8 @@ IFK_API size_t ifk_q8_wgrad_workspace(int64_t rows, int64_t n_out, int64_t n_in,
  * (bf16 or fp32).  accumulate != 0 adds to dW and db instead of overwriting
  * them.  The products are exact and summed in fp32 in either delta type (an fp32
  * delta is taken apart into three bf16 terms); the result does not depend on
- * the run.  rows == 0 gives zeros (or adds nothing).  *d_status (may be NULL)
+ * the run.  With IFK_BF16 | IFK_DELTA_IN_PLACE a delta that is not aligned as
+ * said there is refused (IFK_ERR_ARG).  rows == 0 gives zeros (or adds nothing).  *d_status (may be NULL)
  * receives IFK_ERR_TIMEOUT if a bounded device-side wait gave up; dW is then not
  * valid and holds NaN.  dW and db must not overlap the inputs.
  */

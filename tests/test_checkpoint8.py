@@ -322,3 +322,22 @@ def test_rows_are_unpacked_a_share_at_a_time(precision, size):
     calls.clear()
     hooks._fold_entries([("X", "a", [plain] * 3), ("G", "a", [plain])])
     assert calls == [[("X", "a", [plain] * 3), ("G", "a", [plain])]]
+
+
+def test_a_delta_read_in_place_needs_no_room_for_a_copy():
+    L = _lib.lib()
+    at, rows, n_out, n_in = _lib.BF16 | _lib.DELTA_IN_PLACE, 16384, 4096, 4096
+    full, less = (L.ifk_q8_wgrad_workspace(rows, n_out, n_in, d) for d in (_lib.BF16, at))
+    assert full - less == 2 * rows * n_out and 0 < less < 1 << 26
+    assert L.ifk_q8_wgrad_workspace(rows, n_out, n_in, _lib.F32 | _lib.DELTA_IN_PLACE) == 0
+    need = L.ifk_q8_wgrad_workspace(8, 16, 64, at)
+
+    def wgrad(delta=FAKE, ld=16, dt=at, wsb=need):
+        return L.ifk_q8_wgrad(delta, ld, dt, FAKE, 64, FAKE, 2, 8, 16, 64, FAKE, 64, None, 0, None, FAKE, wsb, None)
+
+    assert wgrad(delta=ctypes.c_void_p(4104)) == _lib.ERR_ARG
+    assert wgrad(ld=20) == _lib.ERR_ARG
+    assert wgrad(ld=15) == _lib.ERR_SHAPE
+    assert wgrad(dt=_lib.F32 | _lib.DELTA_IN_PLACE) == _lib.ERR_DTYPE
+    assert wgrad(wsb=need - 1) == _lib.ERR_WORKSPACE
+    assert wgrad(dt=_lib.BF16, wsb=need) == _lib.ERR_WORKSPACE  # any alignment: room for the copy

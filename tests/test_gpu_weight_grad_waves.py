@@ -94,3 +94,20 @@ def test_long_sums_do_not_drift(dtype):
     bound = 1.05 * (ADDS + accumulators(rows, dtype) / 2 + 1) * U
     assert float(err.abs().max()) <= bound
     assert abs(float(err.mean())) <= 2e-6
+
+
+def test_transient_memory_of_an_aligned_delta():
+    """16384 rows of bf16, 2048 to 2048: outputs and the shares of cut tiles, and no copy of delta (67 MB)."""
+    delta, q = inputs(16384, 2048, 2048, BF)
+    c8().weight_grad(delta, q, bias=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    dW, db = c8().weight_grad(delta, q, bias=True)
+    peak = torch.cuda.max_memory_allocated() - before
+    parts = 2 * 74 * 256 * 256 * 4
+    assert peak <= dW.nbytes + db.nbytes + parts + 592 * 2048 * 4 + (1 << 21)
+    odd = torch.empty(16384, 2049, dtype=BF, device="cuda")[:, :2048]
+    odd.copy_(delta)
+    other, _ = c8().weight_grad(odd, q)
+    assert torch.equal(other, dW)
