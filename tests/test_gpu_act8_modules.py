@@ -181,3 +181,24 @@ def test_a_captured_training_step():
         graph.replay()
         got = [t.clone() for t in out]
         assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+def test_recomputed_and_offloaded_activations():
+    """The same gradients, bit for bit, with the block recomputed in its backward pass and with the saved
+    rows kept on the host meanwhile."""
+    from torch.utils.checkpoint import checkpoint
+    _, c8, _ = mods()
+    torch.manual_seed(0)
+    model = c8.convert(nn.Sequential(nn.LayerNorm(64), nn.Linear(64, 128), nn.GELU(), nn.Linear(128, 64))).cuda()
+    x = randn(6, 30, 64).requires_grad_()
+
+    def grads(run):
+        with torch.autocast("cuda", dtype=BF):
+            loss = run(x).float().square().mean()
+        return torch.autograd.grad(loss, [x, *model.parameters()])
+
+    want = grads(model)
+    assert all(torch.equal(p, q) for p, q in zip(grads(lambda t: checkpoint(model, t, use_reentrant=False)), want))
+    with torch.autograd.graph.save_on_cpu():
+        got = grads(model)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -480,3 +480,38 @@ def test_calls_on_two_streams_at_once():
     for k in range(2):
         for out in got[k]:
             assert all(torch.equal(p, q) for p, q in zip(out, want[k]))
+
+
+@pytest.mark.parametrize("xd", [BF, F4])
+@pytest.mark.parametrize("rows,n,pad", [(40, 768, 0), (1300, 1000, 0), (33, 1001, 0), (9, 4096, 1), (700, 96, 3),
+                                        (3, 9000, 0), (2, 17000, 0)])
+def test_layer_norm_of_a_bf16_model(rows, n, pad, xd):
+    """bf16 weights and a missing bias, on rows of either type, aligned or not: the bits of the same
+    weights in fp32, forward (with and without 8-bit rows) and backward."""
+    x = buffer(rows, n, xd, pad, spread=4.0)
+    dy = buffer(rows, n, xd, pad, seed=1, spread=1.0)
+    wb = (1 + 0.1 * buffer(1, n, F4, seed=4, spread=1.0)[0]).to(BF)
+    bb = (0.1 * buffer(1, n, F4, seed=5, spread=1.0)[0]).to(BF)
+    for w, b in ((wb, bb), (wb, None), (None, bb)):
+        f = [None if t is None else t.float() for t in (w, b)]
+        for checkpoint in (False, True):
+            y, s = c8().layer_norm_forward(x, w, b, save=True, checkpoint=checkpoint)
+            yy, ss = c8().layer_norm_forward(x, *f, save=True, checkpoint=checkpoint)
+            assert torch.equal(y, yy) and torch.equal(s.mean, ss.mean) and torch.equal(s.rstd, ss.rstd)
+            if checkpoint:
+                assert torch.equal(s.q8.codes, ss.q8.codes) and torch.equal(s.q8.scales, ss.q8.scales)
+            for p, q in zip(c8().layer_norm_backward(dy, s, w), c8().layer_norm_backward(dy, ss, f[0])):
+                assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [BF, F4])
+def test_weight_grad_of_a_slice_of_rows(dtype):
+    """Rows from the middle of a batch: codes and scales that start anywhere, and are not copied."""
+    q = c8().quantize_rows(buffer(400, 40, BF))
+    delta = buffer(400, 72, dtype, seed=2, scale=1e-3)
+    for lo, hi in ((0, 400), (3, 130), (129, 130), (255, 400), (7, 7)):
+        part = q[lo:hi]
+        dW, db = c8().weight_grad(delta[lo:hi], part, bias=True)
+        check_wgrad(dW, db, delta[lo:hi], part)
+        own = c8().Q8Rows(part.codes.clone(), part.scales.clone(), 40)
+        assert torch.equal(dW, c8().weight_grad(delta[lo:hi].clone(), own)[0])
