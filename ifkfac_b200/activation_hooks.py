@@ -116,7 +116,7 @@ class RawActivationHooks:
 
     _SEQ_SUBSAMPLE: int = 2048
     # values unpacked from 8 bits at a time, for one fold call; a chunk (one pass's rows of a layer) is not split
-    _UNPACK_BYTES: int = 1 << 30
+    _UNPACK_BYTES: int = 1 << 29
 
     def __init__(self, model: nn.Module, damping: float = 1e-2, max_out_dim: int = 0,
                  augment_bias: bool = False, max_conv_rows: int = 512,
