@@ -112,6 +112,8 @@ class RawActivationHooks:
     their fold; next to a ``Linear8`` layer, X is that layer's own 8-bit input, kept
     once for the weight gradient and the factor.  The factors are then those of the
     rounded rows.  Conv2d inputs, which the folds read through im2col, stay images.
+    Layers that read one tensor each keep 8-bit rows of it, where the hooks otherwise
+    keep one reference.
     """
 
     _SEQ_SUBSAMPLE: int = 2048

@@ -13,7 +13,7 @@ group and integer codes, so every value is exact in bf16 and fp32).
   weight and bias gradients, from the saved input or its 8-bit rows;
 * :class:`Linear8`, :class:`LayerNorm8`: ``nn.Linear`` / ``nn.LayerNorm`` that
   save their input in 8 bits for the backward pass, and :func:`convert`, which
-  puts them in a model's place of its own.
+  puts them in the place of a model's own.
 
 ``RawActivationHooks(capture_8bit=True)`` (and ``IFKFAC``) keeps its pending rows
 this way; next to a :class:`Linear8` it shares that layer's rows.
@@ -242,7 +242,9 @@ def weight_grad(delta: torch.Tensor, q: Q8Rows, bias: bool = False, out: Optiona
     """(dW, db) of a linear layer y = x W^T + b: dW = delta^T X (n_out x n_in fp32)
     from the 8-bit rows of X, and with ``bias`` (or ``out_bias``) db = the column sums
     of delta, else None.  ``out`` / ``out_bias`` receive them; with ``accumulate`` they
-    are added to (gradient accumulation), and both that are wanted must be given."""
+    are added to (gradient accumulation), and both that are wanted must be given.
+    If a wait on the device gave up, dW holds NaN, and ``status`` (a device int32,
+    optional) IFK_ERR_TIMEOUT."""
     dev = _need_cuda(delta, *q.tensors(), out, out_bias, status)
     delta, rows, n_out, ld = _rows2d(delta, "delta")
     dt = _code(delta.dtype)
@@ -356,7 +358,8 @@ def layer_norm_backward(dy: torch.Tensor, saved: LayerNormSaved, weight: Optiona
                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw, db) of :func:`layer_norm_forward`: dx in the input's dtype, dw and db
     fp32 (None without ``weight_grads``).  ``status`` (a device int32, optional)
-    receives IFK_ERR_TIMEOUT if a wait on the device gave up."""
+    receives IFK_ERR_TIMEOUT if a wait on the device gave up; dw, db and the rows of dx
+    that were left are then NaN."""
     dev = _need_cuda(dy, saved.data, weight, status)
     dy, rows, n, ld = _rows2d(dy, "dy")
     dt, xdt = _code(dy.dtype), _code(saved.x_dtype)
@@ -449,7 +452,8 @@ class Linear8(nn.Linear):
     Forward and input gradient are ``nn.Linear``'s (in the autocast dtype under
     autocast); the weight and bias gradients come from :func:`weight_grad`, summed in
     fp32.  While hooks that capture in 8 bits are attached (``share_rows``), ``take_rows``
-    hands each set of them the rows of the forward pass, so they are quantised once."""
+    hands each set of them the rows of the forward pass, so they are quantised once.
+    Layers that read the same tensor each keep 8-bit rows of their own."""
 
     _share_rows = 0                       # sets of hooks that want the rows
     _pass: Optional[_PassRows] = None

@@ -15,11 +15,13 @@
 // beforehand into three bf16 terms (8 + 8 + 8 bits, by truncation: exact), and each 64
 // rows take three steps.
 //
-// The tensor core truncates as it adds to the accumulator, so a long sum drifts
-// towards zero by about 7e-9 of itself a tcgen05.mma; after CHUNK steps (120 of them)
-// the accumulator is therefore added to dW in L2 (red.global.add, rounded to nearest;
-// one thread owns an element, so the order is fixed) while the next chunk goes to the
-// other half of TMEM.
+// The tensor core truncates as it adds to the accumulator, so a long sum drifts towards
+// zero: positive codes and deltas over 16384 rows come out 6.1e-5 low, over 65536 rows
+// 3.5e-4 (random signs, 16384 rows: 7e-6).  After CHUNK steps (120 tcgen05.mma) the
+// accumulator is therefore added to dW in L2 (red.global.add, rounded to nearest; one
+// thread owns an element, so the order is fixed) while the next chunk goes to the other
+// half of TMEM: 1.1e-6 low in bf16 at either length, 1.5e-6 at most; in the three terms
+// of an fp32 delta 4e-8, 7e-7 at most.
 //
 // Work: whole waves of tiles first, every cluster a tile at a time; the tiles that
 // are left over are cut along the rows into equal shares for all clusters.  A share
@@ -30,7 +32,8 @@
 // out, the tile out and into the tensor core, delta's half in and twice out), 765 clocks
 // where the tensor core needs 512.  Measured: 16384 x 4096 x 4096 bf16 435 to 470 us (1.2
 // PFLOP/s at the 1.5 GHz that the card's power allows) and 36 us for db's sums and the
-// join; 8192 x 768 x 2304 34 + 16 us (49 in all); one row of 2048 x 8192 17 us (67 MB written);
+// join, 470 to 485 us in all where a graph's calls follow one another and 545 to 572 us
+// with every call's inputs from memory; 8192 x 768 x 2304 34 + 16 us (49 in all); one row of 2048 x 8192 17 us (67 MB written);
 // 8192 x 4096 x 4096 fp32 720 to 750 us in all.  A launch's fixed part is about 6 us: set-up 1, the
 // first loads 2, the last accumulator's stores 2, the pair's last meeting 1.
 #include <cuda.h>

@@ -79,9 +79,9 @@ def test_long_sums_do_not_drift(dtype):
     """65536 rows of positive codes and deltas, 74 tiles: 35 accumulators a tile (103 in three
     terms).  Of a sum that grows evenly the average partial sum is half of it, so the bound above
     halves; rows of 1/2 to 1 and 1 to 2 keep every partial sum within 5% of even growth.
-    A single accumulator over all rows loses 7e-9 of itself a product: 2.9e-5, or three
-    times that in three terms.  The mean loss, whose sign does not change, stays under 2e-6:
-    60 times 7e-9 = 4.2e-7 in an accumulator, and the additions between them round to nearest."""
+    The mean loss is the truncations' alone, as the additions between accumulators round to
+    nearest: it stays under 2e-6.  (Measured: 1.1e-6 in bf16, 4e-8 in three terms; with one
+    accumulator over all rows 3.5e-4 in either type.)"""
     rows, n_in, n_out = 65536, 512, 9472
     g = torch.Generator(device="cuda").manual_seed(3)
     q = c8().quantize_rows(torch.rand(rows, n_in, generator=g, device="cuda") + 1)
