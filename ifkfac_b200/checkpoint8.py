@@ -420,7 +420,7 @@ class _LinearQ8(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
-_HOOKS = tuple(k for k in nn.Module().__dict__ if "_hooks" in k)
+_HOOKS = tuple(k for k, v in nn.Module().__dict__.items() if "_hook" in k and isinstance(v, dict))
 
 
 def _take_over(new: nn.Module, m: nn.Module) -> nn.Module:
@@ -428,7 +428,7 @@ def _take_over(new: nn.Module, m: nn.Module) -> nn.Module:
     for k, v in m.__dict__.items():
         if k in ("_parameters", "_buffers", "_modules", "_non_persistent_buffers_set"):
             new.__dict__[k] = v.copy()
-        elif k not in _HOOKS and k != "forward":
+        elif k not in _HOOKS and k not in ("_is_full_backward_hook", "forward"):
             new.__dict__[k] = v
     return new
 
@@ -478,11 +478,11 @@ class Linear8(nn.Linear):
         self._share_rows = max(self._share_rows - 1, 0)
         self._pass = None
 
-    def take_rows(self, out: torch.Tensor) -> Optional[Q8Rows]:
-        """The rows of the forward pass whose output is ``out``, for one set of hooks; None when
-        that pass had none, or another one (a thread's) has come since."""
+    def take_rows(self, out: Optional[torch.Tensor] = None) -> Optional[Q8Rows]:
+        """The rows of the forward pass whose output is ``out`` (None: of the last one), for one
+        set of hooks; None when that pass had none, or another one (a thread's) has come since."""
         p = self._pass
-        if p is None or p.rows is None or p.out() is not out:
+        if p is None or p.rows is None or (out is not None and p.out() is not out):
             return None
         p.left -= 1
         if p.left <= 0 and self._pass is p:
@@ -536,6 +536,8 @@ class LayerNorm8(nn.LayerNorm):
     dtype, which costs nothing where only Linear layers read it (they would cast it), but is
     a rounding where it is a residual stream itself; with ``autocast_output=False`` it is
     fp32 there, as nn.LayerNorm's."""
+
+    autocast_output = True
 
     def __init__(self, normalized_shape, *args, autocast_output: bool = True, **kwargs):
         super().__init__(normalized_shape, *args, **kwargs)

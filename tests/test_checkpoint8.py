@@ -341,3 +341,15 @@ def test_a_delta_read_in_place_needs_no_room_for_a_copy():
     assert wgrad(dt=_lib.F32 | _lib.DELTA_IN_PLACE) == _lib.ERR_DTYPE
     assert wgrad(wsb=need - 1) == _lib.ERR_WORKSPACE
     assert wgrad(dt=_lib.BF16, wsb=need) == _lib.ERR_WORKSPACE  # any alignment: room for the copy
+
+
+def test_a_layer_made_of_a_hooked_one_starts_without_hooks():
+    m = nn.Linear(20, 4)
+    m.register_full_backward_hook(lambda *a: None)
+    new = c8.Linear8.from_linear(m)
+    assert new.weight is m.weight and not new._backward_hooks and new._is_full_backward_hook is None
+    new._pass = c8._PassRows(_rows(), torch.zeros(2), 1)
+    assert new.take_rows().rows == 4 and new.take_rows() is None   # without an output: the last pass's
+    bare = nn.Linear(20, 4)
+    bare.register_full_backward_hook(lambda *a: None).remove()
+    assert type(c8.convert(nn.Sequential(bare))[0]) is c8.Linear8  # its hooks are gone: nothing to lose
